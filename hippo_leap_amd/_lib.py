@@ -15,6 +15,9 @@ HL_OK, HL_EINVAL, HL_ECAPACITY, HL_EUNSUPPORTED, HL_EHIP, HL_ECAPTURE = 0, -1, -
 HL_F32, HL_F16, HL_BF16, HL_FP8 = 0, 1, 2, 3
 HL_ROPE_HALF_SPLIT, HL_ROPE_INTERLEAVED = 0, 1
 HL_KV_COLMAJOR, HL_KV_TILED32, HL_KV_PAGED32 = 0, 1, 2
+HL_ACT_COLMAJOR, HL_ACT_TOKENMAJOR = 0, 1
+HL_ROPE_SCALE_NONE, HL_ROPE_SCALE_LINEAR, HL_ROPE_SCALE_LLAMA3, HL_ROPE_SCALE_YARN = 0, 1, 2, 3
+HL_MAX_ROPE_DIM = 256
 HL_GGML_F16, HL_GGML_Q5_0, HL_GGML_Q5_1, HL_GGML_Q8_0 = 1, 6, 7, 8
 HL_GGML_Q2_K, HL_GGML_Q3_K, HL_GGML_Q4_K, HL_GGML_Q5_K, HL_GGML_Q6_K = 10, 11, 12, 13, 14
 HL_GGML_IQ4_NL = 20
@@ -117,6 +120,47 @@ class PrefillArgs(ctypes.Structure):
     ]
 
 
+class ChunkBatch(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int), ("n_tokens", c_int), ("max_new", c_int), ("max_kv", c_int),
+        ("q_start", c_void_p), ("kv_lens", c_void_p),
+        ("n_head_kv", c_int), ("head_dim", c_int), ("kv_dtype", c_int), ("n_pages", c_int),
+        ("k_pages", c_void_p), ("v_pages", c_void_p), ("block_table", c_void_p), ("blocks_per_seq", c_int),
+    ]
+
+
+class AttnChunkArgs(ctypes.Structure):
+    _fields_ = [
+        ("seqs", ChunkBatch), ("n_head", c_int), ("io_dtype", c_int), ("act_layout", c_int),
+        ("q", c_void_p), ("out", c_void_p), ("q_stride", c_longlong), ("out_stride", c_longlong),
+        ("scale", c_float), ("window", c_int), ("n_sink", c_int), ("num_splits", c_int),
+    ]
+
+
+class RopeScaling(ctypes.Structure):
+    _fields_ = [("kind", c_int)] + [(n, c_float) for n in ("factor", "original_len", "low_freq", "high_freq",
+                                                          "beta_fast", "beta_slow", "attn_factor")]
+
+
+class RopeFreqs(ctypes.Structure):
+    _fields_ = [("rope_dim", c_int), ("gain", c_float), ("turns_hi", c_float * (HL_MAX_ROPE_DIM // 2)),
+                ("turns_lo", c_float * (HL_MAX_ROPE_DIM // 2))]
+
+
+class RopeStoreChunkArgs(ctypes.Structure):
+    _fields_ = [
+        ("seqs", ChunkBatch), ("n_head", c_int), ("io_dtype", c_int), ("act_layout", c_int),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_out", c_void_p),
+        ("q_stride", c_longlong), ("k_stride", c_longlong), ("v_stride", c_longlong), ("q_out_stride", c_longlong),
+        ("rope_style", c_int), ("eps", c_float), ("q_norm_w", c_void_p), ("k_norm_w", c_void_p),
+        ("freqs", RopeFreqs),
+    ]
+
+
+class KvPages(ctypes.Structure):
+    _fields_ = [("n_pools", c_int), ("n_pages", c_int), ("page_bytes", c_size_t), ("pools", ctypes.POINTER(c_void_p))]
+
+
 # name -> (restype, argtypes); every symbol include/hl_attn.h declares.
 SIGNATURES = {
     "hl_last_error": (ctypes.c_char_p, []),
@@ -191,6 +235,19 @@ SIGNATURES = {
                                              ctypes.POINTER(c_int), c_void_p]),
     "hl_probe_stream_read": (c_int, [c_void_p, c_size_t, c_int, c_void_p, c_void_p]),
     "hl_probe_stream_read_ex": (c_int, [c_void_p, c_size_t, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "hl_attn_chunk_workspace_bytes": (c_size_t, [ctypes.POINTER(AttnChunkArgs)]),
+    "hl_attn_chunk": (c_int, [ctypes.POINTER(AttnChunkArgs), c_void_p, c_size_t, c_void_p]),
+    "hl_rope_freqs_init": (c_int, [ctypes.POINTER(RopeFreqs), c_int, c_float, ctypes.POINTER(RopeScaling)]),
+    "hl_rope_store_chunk": (c_int, [ctypes.POINTER(RopeStoreChunkArgs), c_void_p]),
+    "hl_kv_pages_copy": (c_int, [ctypes.POINTER(KvPages), c_void_p, c_int, c_void_p]),
+    "hl_page_pool_create": (c_int, [ctypes.POINTER(c_void_p), c_int]),
+    "hl_page_pool_destroy": (None, [c_void_p]),
+    "hl_page_pool_free_count": (c_int, [c_void_p]),
+    "hl_page_pool_refs": (c_int, [c_void_p, c_int]),
+    "hl_page_pool_extend": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "hl_page_pool_fork": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int]),
+    "hl_page_pool_release": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int]),
+    "hl_page_pool_compact": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, ctypes.POINTER(c_int)]),
     "hl_kv_cache_to_f32": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
 }
 

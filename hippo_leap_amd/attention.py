@@ -25,9 +25,11 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import (HL_BF16, HL_F16, HL_F32, HL_FP8, HL_KV_COLMAJOR, HL_KV_PAGED32,  # noqa: F401
-                   HL_KV_TILED32, HL_ROPE_HALF_SPLIT, DecodeArgs, PrefillArgs, RopeStoreArgs,
-                   HL_OK, check)
+from ._lib import (HL_ACT_COLMAJOR, HL_ACT_TOKENMAJOR, HL_BF16, HL_F16, HL_F32, HL_FP8,  # noqa: F401
+                   HL_KV_COLMAJOR, HL_KV_PAGED32, HL_KV_TILED32, HL_ROPE_HALF_SPLIT, HL_ROPE_INTERLEAVED,
+                   HL_ROPE_SCALE_LINEAR, HL_ROPE_SCALE_LLAMA3, HL_ROPE_SCALE_NONE, HL_ROPE_SCALE_YARN,
+                   AttnChunkArgs, ChunkBatch, DecodeArgs, KvPages, PrefillArgs, RopeFreqs, RopeScaling,
+                   RopeStoreArgs, RopeStoreChunkArgs, HL_OK, check)
 
 _DT = {torch.float32: HL_F32, torch.float16: HL_F16, torch.bfloat16: HL_BF16,
        torch.float8_e4m3fn: HL_FP8, torch.uint8: HL_FP8}
@@ -411,3 +413,197 @@ def workspace(nbytes: int, device="cuda") -> torch.Tensor | None:
     if nbytes <= 0:
         return None
     return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+
+# ---------------------------------------------------------------------------
+# Chunks of new tokens over paged caches
+# ---------------------------------------------------------------------------
+def chunk_batch(k_pages, v_pages, block_table, q_start, kv_lens, n_tokens, max_new, max_kv, n_head_kv,
+                head_dim) -> ChunkBatch:
+    """The new tokens of B sequences and their pages (hl_chunk_batch).  Pools of
+    [n_head_kv][head_dim][32] pages; block_table int32 [B, blocks_per_seq],
+    q_start int32 [B + 1], kv_lens int32 [B] (each sequence's length with its
+    new tokens), all on the device and read when the kernels run."""
+    for name, t in (("block_table", block_table), ("q_start", q_start), ("kv_lens", kv_lens)):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise _lib.HLError(_lib.HL_EINVAL, f"{name} must be a contiguous int32 tensor")
+    if block_table.dim() != 2 or q_start.numel() != block_table.shape[0] + 1 or kv_lens.numel() != block_table.shape[0]:
+        raise _lib.HLError(_lib.HL_EINVAL, "block_table is [B, blocks_per_seq], q_start [B + 1], kv_lens [B]")
+    page = n_head_kv * head_dim * 32
+    if (k_pages.dtype != v_pages.dtype or k_pages.numel() != v_pages.numel() or k_pages.numel() % page
+            or not k_pages.is_contiguous() or not v_pages.is_contiguous()):
+        raise _lib.HLError(_lib.HL_EINVAL, "the pools must be contiguous, of one type and whole pages")
+    s = ChunkBatch()
+    s.batch, s.blocks_per_seq = block_table.shape
+    s.n_tokens, s.max_new, s.max_kv = n_tokens, max_new, max_kv
+    s.q_start, s.kv_lens, s.block_table = _p(q_start), _p(kv_lens), _p(block_table)
+    s.n_head_kv, s.head_dim, s.kv_dtype = n_head_kv, head_dim, dtype_code(k_pages)
+    s.n_pages = k_pages.numel() // page
+    s.k_pages, s.v_pages = _p(k_pages), _p(v_pages)
+    s._tensors = (k_pages, v_pages, block_table, q_start, kv_lens)
+    return s
+
+
+def _act(t, rows, n_tokens, layout, name):
+    """(pointer, stride) of an activation tensor: [rows, n_tokens] column-major
+    or [n_tokens, rows] token-major, its inner dimension contiguous."""
+    want = (rows, n_tokens) if layout == HL_ACT_COLMAJOR else (n_tokens, rows)
+    if tuple(t.shape) != want or (want[1] > 1 and t.stride(1) != 1):
+        raise _lib.HLError(_lib.HL_EINVAL, f"{name} must be {want} with its last dimension contiguous")
+    return _p(t), t.stride(0) if want[0] > 1 else 0
+
+
+def attn_chunk_args(batch: ChunkBatch, q, out, n_head, act_layout=HL_ACT_COLMAJOR, scale=0.0, window=0, n_sink=0,
+                    num_splits=0) -> AttnChunkArgs:
+    """Arguments of hl_attn_chunk; q and out of one type and layout."""
+    if q.dtype != out.dtype:
+        raise _lib.HLError(_lib.HL_EINVAL, "q and out must have one type")
+    a = AttnChunkArgs()
+    a.seqs, a.n_head, a.io_dtype, a.act_layout = batch, n_head, dtype_code(q), act_layout
+    rows = n_head * batch.head_dim
+    a.q, a.q_stride = _act(q, rows, batch.n_tokens, act_layout, "q")
+    a.out, a.out_stride = _act(out, rows, batch.n_tokens, act_layout, "out")
+    a.scale, a.window, a.n_sink, a.num_splits = scale, window, n_sink, num_splits
+    a._tensors = (batch, q, out)
+    return a
+
+
+def attn_chunk_workspace_bytes(args: AttnChunkArgs) -> int:
+    return int(_lib.load().hl_attn_chunk_workspace_bytes(ctypes.byref(args)))
+
+
+def attn_chunk_workspace(args: AttnChunkArgs, device="cuda", stream=None):
+    """Allocates and zero-initialises a workspace of hl_attn_chunk (None if not needed)."""
+    nbytes = attn_chunk_workspace_bytes(args)
+    if nbytes <= 0:
+        return None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    check(_lib.load().hl_attn_decode_workspace_init(ws.data_ptr(), nbytes, _stream(stream)))
+    return ws
+
+
+def attn_chunk(args: AttnChunkArgs, workspace=None, stream=None) -> None:
+    """hl_attn_chunk: attention of the chunk's tokens over their sequences' pages."""
+    ws = workspace.data_ptr() if workspace is not None else None
+    nbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    check(_lib.load().hl_attn_chunk(ctypes.byref(args), ws, nbytes, _stream(stream)))
+
+
+def rope_scaling(kind=HL_ROPE_SCALE_NONE, factor=1.0, original_len=0.0, low_freq=0.0, high_freq=0.0, beta_fast=0.0,
+                 beta_slow=0.0, attn_factor=0.0) -> RopeScaling:
+    return RopeScaling(kind, factor, original_len, low_freq, high_freq, beta_fast, beta_slow, attn_factor)
+
+
+def rope_freqs(rope_dim: int, rope_base: float, scaling: RopeScaling | None = None) -> RopeFreqs:
+    """The table of rotary frequencies (hl_rope_freqs_init); host only."""
+    f = RopeFreqs()
+    check(_lib.load().hl_rope_freqs_init(ctypes.byref(f), rope_dim, rope_base,
+                                         ctypes.byref(scaling) if scaling is not None else None))
+    return f
+
+
+def rope_store_chunk_args(batch: ChunkBatch, q, k, v, q_out, n_head, rope_base, rope_dim=0,
+                          rope_style=HL_ROPE_HALF_SPLIT, scaling=None, q_norm_w=None, k_norm_w=None, eps=1e-6,
+                          act_layout=HL_ACT_COLMAJOR, freqs=None) -> RopeStoreChunkArgs:
+    """Arguments of hl_rope_store_chunk.  rope_dim 0: the whole head; freqs: a
+    table made before (rope_base, rope_dim and scaling are then not used)."""
+    if not q.dtype == k.dtype == v.dtype == q_out.dtype:
+        raise _lib.HLError(_lib.HL_EINVAL, "q, k, v and q_out must have one type")
+    a = RopeStoreChunkArgs()
+    a.seqs, a.n_head, a.io_dtype, a.act_layout = batch, n_head, dtype_code(q), act_layout
+    rows, rows_kv, n = n_head * batch.head_dim, batch.n_head_kv * batch.head_dim, batch.n_tokens
+    a.q, a.q_stride = _act(q, rows, n, act_layout, "q")
+    a.k, a.k_stride = _act(k, rows_kv, n, act_layout, "k")
+    a.v, a.v_stride = _act(v, rows_kv, n, act_layout, "v")
+    a.q_out, a.q_out_stride = _act(q_out, rows, n, act_layout, "q_out")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != batch.head_dim or not w.is_contiguous()):
+            raise _lib.HLError(_lib.HL_EINVAL, "norm weights are contiguous fp32 [head_dim]")
+    a.q_norm_w, a.k_norm_w, a.eps, a.rope_style = _p(q_norm_w), _p(k_norm_w), eps, rope_style
+    a.freqs = freqs if freqs is not None else rope_freqs(rope_dim or batch.head_dim, rope_base, scaling)
+    a._tensors = (batch, q, k, v, q_out, q_norm_w, k_norm_w)
+    return a
+
+
+def rope_store_chunk(args: RopeStoreChunkArgs, stream=None) -> None:
+    """hl_rope_store_chunk: qkNorm, rotation and the store into the pages."""
+    check(_lib.load().hl_rope_store_chunk(ctypes.byref(args), _stream(stream)))
+
+
+def kv_pages_args(pools) -> KvPages:
+    """The K and V pools of every layer (tensors [n_pages, ...] of one size)."""
+    pools = list(pools)
+    if not pools or any(p.shape != pools[0].shape or p.dtype != pools[0].dtype or not p.is_contiguous() for p in pools):
+        raise _lib.HLError(_lib.HL_EINVAL, "the pools must be contiguous [n_pages, ...] tensors of one type and size")
+    a = KvPages()
+    a.n_pools, a.n_pages = len(pools), pools[0].shape[0]
+    a.page_bytes = pools[0].numel() // max(1, a.n_pages) * pools[0].element_size()
+    a._pointers = (ctypes.c_void_p * len(pools))(*(_p(p) for p in pools))
+    a.pools = ctypes.cast(a._pointers, ctypes.POINTER(ctypes.c_void_p))
+    a._tensors = pools
+    return a
+
+
+def kv_pages_copy(args: KvPages, moves: torch.Tensor, stream=None) -> None:
+    """hl_kv_pages_copy: page to becomes page from in every pool, for each row
+    (from, to) of the host int32 tensor moves [n, 2]."""
+    if moves.is_cuda or moves.dtype != torch.int32 or not moves.is_contiguous() or moves.numel() % 2:
+        raise _lib.HLError(_lib.HL_EINVAL, "moves must be a contiguous int32 host tensor [n, 2]")
+    check(_lib.load().hl_kv_pages_copy(ctypes.byref(args), moves.data_ptr(), moves.numel() // 2, _stream(stream)))
+
+
+class PagePool:
+    """Which pages are free and who shares them (hl_page_pool_*): host state.
+    Tables are contiguous int32 host tensors, -1 where there is no page."""
+
+    def __init__(self, n_pages: int):
+        self._h = ctypes.c_void_p()
+        check(_lib.load().hl_page_pool_create(ctypes.byref(self._h), n_pages))
+
+    def __del__(self):
+        if getattr(self, "_h", None) and _lib._lib is not None:
+            _lib._lib.hl_page_pool_destroy(self._h)
+            self._h = None
+
+    @staticmethod
+    def _table(t):
+        if t.is_cuda or t.dtype != torch.int32 or not t.is_contiguous():
+            raise _lib.HLError(_lib.HL_EINVAL, "tables are contiguous int32 host tensors")
+        return t.data_ptr()
+
+    @property
+    def free(self) -> int:
+        return _lib.load().hl_page_pool_free_count(self._h)
+
+    def refs(self, page: int) -> int:
+        n = _lib.load().hl_page_pool_refs(self._h, page)
+        if n < 0:
+            check(n)
+        return n
+
+    def extend(self, table, old_len: int, new_len: int):
+        """Positions old_len .. new_len - 1 made writable; the (from, to) copy
+        that this needs first, or None."""
+        move = (ctypes.c_int32 * 2)()
+        check(_lib.load().hl_page_pool_extend(self._h, self._table(table), table.numel(), old_len, new_len, move))
+        return (move[0], move[1]) if move[0] >= 0 else None
+
+    def fork(self, table, new_table, length: int) -> None:
+        """new_table shares table's pages of the first `length` positions."""
+        if new_table.numel() != table.numel():
+            raise _lib.HLError(_lib.HL_EINVAL, "the tables must have one size")
+        check(_lib.load().hl_page_pool_fork(self._h, self._table(table), self._table(new_table), table.numel(), length))
+
+    def release(self, table, first: int = 0, count: int | None = None) -> None:
+        """Gives back blocks first .. first + count - 1 (default: the rest)."""
+        n = table.numel() - first if count is None else count
+        check(_lib.load().hl_page_pool_release(self._h, self._table(table), table.numel(), first, n))
+
+    def compact(self, tables, max_moves: int | None = None) -> torch.Tensor:
+        """Moves pages to the lowest indices; tables [n, blocks] change to match.
+        Returns the moves [n, 2] for kv_pages_copy."""
+        moves = torch.empty(tables.numel() if max_moves is None else max_moves, 2, dtype=torch.int32)
+        n = ctypes.c_int(0)
+        check(_lib.load().hl_page_pool_compact(self._h, self._table(tables), tables.shape[0], tables.shape[1],
+                                               moves.data_ptr(), moves.shape[0], ctypes.byref(n)))
+        return moves[:n.value].contiguous()

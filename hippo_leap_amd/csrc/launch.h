@@ -258,6 +258,23 @@ bool linear_quant_norm_launch(int nmat, const void* const* w, float* const* y, c
                               float* xsum, const float* x, const float* res, const float* nrm, float eps,
                               hipStream_t stream);
 
+// ---- chunks of new tokens over paged caches --------------------------------
+// Attention (chunk.hip).  Workspace: kChunkSlots arrival counters, partials.
+constexpr int kChunkSlots = 4096;
+struct ChunkAttnPlan {
+  int rb, rows;      // 16-row blocks, rows of a workgroup
+  bool direct;       // every chunk fits one workgroup's rows: work item = sequence
+  int items;         // row blocks of all sequences, at most
+  int tps, splits;   // 32-key tiles per split, most splits of a row block
+  size_t ws_bytes;
+};
+void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan);
+hipError_t chunk_attn_launch(const hl_attn_chunk_args* a, const ChunkAttnPlan* plan, void* ws, hipStream_t stream);
+// qkNorm, rotation and store (rope_chunk.hip).
+hipError_t rope_chunk_launch(const hl_rope_store_chunk_args* a, hipStream_t stream);
+// Page copies (pages.hip): checked moves.
+hipError_t pages_copy_launch(const hl_kv_pages* pages, const int32_t* moves, int n_moves, hipStream_t stream);
+
 // Whether two buffers share a byte.
 inline bool overlaps(const void* a, size_t abytes, const void* b, size_t bbytes) {
   const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;

@@ -728,6 +728,193 @@ int hl_forward_decode_timed(const hl_model_desc* model, hl_kv_cache_desc* cache,
                             float* logits, int32_t* next_token_dev, int32_t* next_token,
                             float* gpu_ms, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Serving over paged caches (HL_KV_PAGED32): chunks of new tokens of several */
+/* sequences, rotary positions for long contexts, and the pages themselves.   */
+/* Extends the reference, whose prefill starts at position 0 and whose cache  */
+/* is one block per sequence (naive.nim:3967-3976, 3912-3931).               */
+/* ------------------------------------------------------------------------ */
+
+/* Layout of a chunk's activations (q, k, v, out): row r of n_head*head_dim,
+ * token t of n_tokens, with a stride in elements (0 = dense).              */
+enum {
+  HL_ACT_COLMAJOR = 0,     /* (r, t) at r * stride + t: hl_prefill_args's     */
+  HL_ACT_TOKENMAJOR = 1    /* (r, t) at t * stride + r: hl_decode_args's      */
+};
+
+/* The new tokens of B sequences and the caches they belong to.  Sequence b's
+ * new tokens are activation tokens q_start[b] .. q_start[b + 1] - 1 (none
+ * where the two are equal) and its last positions: with T of them, token i
+ * is at position kv_lens[b] - T + i.  Tokens before q_start[0] or from
+ * q_start[B] on (padding) are neither read nor written.
+ * q_start, kv_lens and block_table are device memory, read when the kernels
+ * run, so that a captured call can be replayed with other contents.  They
+ * have to keep within the host's bounds: q_start ascending within
+ * [0, n_tokens], chunks of at most max_new tokens, lengths of at most max_kv.
+ * What does not is cut to them (its outputs are then unspecified, and no
+ * access leaves the buffers).  A position whose page lies outside
+ * [0, n_pages) is invisible to attention and not stored.                   */
+typedef struct hl_chunk_batch {
+  int batch;                    /* B, 1 .. 65535                              */
+  int n_tokens;                 /* tokens the activations hold                */
+  int max_new;                  /* longest chunk                              */
+  int max_kv;                   /* longest kv_lens, <= 32 * blocks_per_seq    */
+  const int* q_start;           /* device int[B + 1]                          */
+  const int* kv_lens;           /* device int[B], the chunk included          */
+  int n_head_kv, head_dim;      /* head_dim 64 or 128                         */
+  int kv_dtype;                 /* HL_F16 | HL_BF16 | HL_FP8                  */
+  int n_pages;                  /* pages of each pool                         */
+  void* k_pages;                /* pools of [Hkv][D][32] pages, 16-byte aligned */
+  void* v_pages;
+  const int* block_table;       /* device int[B][blocks_per_seq]              */
+  int blocks_per_seq;
+} hl_chunk_batch;
+
+/* Attention of the new tokens over their sequences' pages (which hold the
+ * new tokens' own k and v: hl_rope_store_chunk before this).  Token at
+ * position i sees positions j <= i; with window > 0 only those with
+ * i - j < window or j < n_sink (the first tokens, which stay visible while
+ * the window slides).  Pages whose positions no token of the chunk sees are
+ * not read, and their table entries may hold anything.  A token that sees
+ * nothing (a position below 0, pages outside the pool) gets zeros.
+ * out = softmax(q . K^T * scale) . V per head, kv head = h / (Hq / Hkv).
+ * Scores, softmax statistics and sums are fp32.  fp32 activations are split
+ * so that their products keep fp32's precision (q and the weights in 3 bf16
+ * or 2 fp16 parts); with fp16 / bf16 activations the weights are rounded
+ * once to the caches' type (fp16 for fp8 caches).  An inf or NaN in k or v
+ * reaches exactly the tokens that see it (an inf of v as a NaN with fp32
+ * activations, whose parts can differ in sign).                            */
+typedef struct hl_attn_chunk_args {
+  hl_chunk_batch seqs;
+  int n_head;                   /* Hq, Hq % Hkv == 0                          */
+  int io_dtype;                 /* of q and out: HL_F32 | HL_F16 | HL_BF16    */
+  int act_layout;               /* HL_ACT_COLMAJOR | HL_ACT_TOKENMAJOR        */
+  const void* q;                /* device; out must not overlap it            */
+  void* out;
+  long long q_stride, out_stride;
+  float scale;                  /* 0 -> 1/sqrtf(D); not negative              */
+  int window;                   /* 0: no window                               */
+  int n_sink;                   /* used with a window only                    */
+  int num_splits;               /* 0 -> chosen to fill the GPU; else at most
+                                   this many workgroups share a token's keys  */
+} hl_attn_chunk_args;
+
+/* Device workspace hl_attn_chunk needs for these args (0: none), 16-byte
+ * aligned: 16 KB of arrival counters, then the partial results of contexts
+ * split over workgroups.  The counters must be zero before the first call
+ * (hl_attn_decode_workspace_init on the fresh workspace); each call leaves
+ * them zero, so chunk calls of any shape may follow one another on one
+ * workspace, graph replays too.  It must not hold other data in between
+ * (hl_attn_decode's partials neither), and calls that overlap in time must
+ * not share it.                                                            */
+size_t hl_attn_chunk_workspace_bytes(const hl_attn_chunk_args* a);
+int hl_attn_chunk(const hl_attn_chunk_args* a, void* workspace, size_t ws_bytes, void* stream);
+
+/* Rotary frequencies, scaled for contexts longer than a model was trained
+ * on.  With f_i = rope_base^(-2i/rope_dim):
+ *   NONE    f_i
+ *   LINEAR  f_i / factor
+ *   LLAMA3  with n = original_len * f_i / 2 pi (turns over the original
+ *           context): f_i where n >= high_freq, f_i / factor where
+ *           n <= low_freq, between them linear in n
+ *   YARN    with i(n) the (real) index whose pair makes n turns over
+ *           original_len: f_i below floor(i(beta_fast)), f_i / factor above
+ *           ceil(i(beta_slow)), between them linear in i; cos and sin are
+ *           multiplied by attn_factor (0 -> 0.1 ln(factor) + 1)            */
+enum { HL_ROPE_SCALE_NONE = 0, HL_ROPE_SCALE_LINEAR = 1, HL_ROPE_SCALE_LLAMA3 = 2, HL_ROPE_SCALE_YARN = 3 };
+typedef struct hl_rope_scaling {
+  int kind;
+  float factor;                 /* >= 1                                       */
+  float original_len;           /* LLAMA3, YARN: positions trained on         */
+  float low_freq, high_freq;    /* LLAMA3: 0 -> 1 and 4                       */
+  float beta_fast, beta_slow;   /* YARN: 0 -> 32 and 1                        */
+  float attn_factor;            /* YARN                                       */
+} hl_rope_scaling;
+
+/* A table of frequencies in turns (angle / 2 pi) per position, as two floats
+ * each: a position's angle is then off by less than 2^-24 of a turn whatever
+ * the position (the reference's fp32 product, naive.nim:3065-3073, is off by
+ * 0.006 rad at position 100000).  Computed once on the host.               */
+typedef struct hl_rope_freqs {
+  int rope_dim;                 /* 0: no rotation                             */
+  float gain;                   /* factor of cos and sin                      */
+  float turns_hi[HL_MAX_ROPE_DIM / 2];
+  float turns_lo[HL_MAX_ROPE_DIM / 2];
+} hl_rope_freqs;
+/* scaling NULL: none. */
+int hl_rope_freqs_init(hl_rope_freqs* freqs, int rope_dim, float rope_base, const hl_rope_scaling* scaling);
+
+/* One launch for the new tokens of B sequences: optional qkNorm of q and k
+ * (naive.nim:2918-2926), rotation of their first rope_dim dims at each
+ * token's position, the rotated q into q_out, k and v into the pages
+ * (rounded to nearest even; fp8 saturating).  k and v are only read; q_out
+ * may be q itself (same stride) and otherwise must not overlap the inputs.
+ * Arithmetic is fp32, q_out is rounded once.                               */
+typedef struct hl_rope_store_chunk_args {
+  hl_chunk_batch seqs;
+  int n_head;
+  int io_dtype;                 /* of q, k, v and q_out                       */
+  int act_layout;
+  const void* q;                /* [Hq*D] rows                                */
+  const void* k;                /* [Hkv*D] rows                               */
+  const void* v;
+  void* q_out;
+  long long q_stride, k_stride, v_stride, q_out_stride;
+  int rope_style;               /* HL_ROPE_HALF_SPLIT | HL_ROPE_INTERLEAVED   */
+  float eps;
+  const float* q_norm_w;        /* optional device [D]                        */
+  const float* k_norm_w;
+  hl_rope_freqs freqs;
+} hl_rope_store_chunk_args;
+int hl_rope_store_chunk(const hl_rope_store_chunk_args* a, void* stream);
+
+/* Page copies: for each move (from, to) of the host list moves[n_moves][2],
+ * page `to` of every pool becomes page `from` (a forked sequence's part-
+ * filled page, a compacted pool's pages).  One launch copies up to 64 pools x
+ * 256 moves.  HL_EINVAL, before anything is launched, for a page outside
+ * [0, n_pages), a page that two moves write, or one that is both written and
+ * read.  The list is consumed before the call returns, and a captured call
+ * keeps it.                                                                */
+typedef struct hl_kv_pages {
+  int n_pools;                  /* K and V of every layer: 2 * n_layer        */
+  int n_pages;
+  size_t page_bytes;            /* n_head_kv * head_dim * 32 * element size; a
+                                   multiple of 16                             */
+  void* const* pools;           /* host array of device pools, 16-byte aligned,
+                                   none overlapping another                   */
+} hl_kv_pages;
+int hl_kv_pages_copy(const hl_kv_pages* pages, const int32_t* moves, int n_moves, void* stream);
+
+/* Which pages are free and how many sequences share each: host state only,
+ * no device memory.  A pool serves one set of page pools (all layers share
+ * one block table).  Tables are host int32[blocks_per_seq] rows, entries -1
+ * where there is no page; the caller uploads them.  A call that fails leaves
+ * the pool and the tables as they were.  Calls on one pool must not overlap. */
+typedef struct hl_page_pool hl_page_pool;
+int hl_page_pool_create(hl_page_pool** pool, int n_pages);
+void hl_page_pool_destroy(hl_page_pool* pool);
+int hl_page_pool_free_count(const hl_page_pool* pool);          /* < 0: pool is null */
+int hl_page_pool_refs(const hl_page_pool* pool, int page);      /* sequences that hold it */
+/* Makes positions old_len .. new_len - 1 of a sequence writable: fresh pages
+ * for the blocks that have none, and a fresh page with a move (from, to) into
+ * move[2] where the block of position old_len is part-filled and shared (copy
+ * on write; move[0] = -1 otherwise).  HL_ECAPACITY when pages run out.       */
+int hl_page_pool_extend(hl_page_pool* pool, int32_t* table, int blocks_per_seq, int old_len, int new_len,
+                        int32_t move[2]);
+/* to becomes a copy of from's first ceil(len / 32) blocks, sharing the pages
+ * (the rest of to is -1); to must hold no pages.                            */
+int hl_page_pool_fork(hl_page_pool* pool, const int32_t* from, int32_t* to, int blocks_per_seq, int len);
+/* Gives back blocks first .. first + count - 1 (a finished sequence's, or
+ * those a window has left behind); their entries become -1.                 */
+int hl_page_pool_release(hl_page_pool* pool, int32_t* table, int blocks_per_seq, int first, int count);
+/* Moves held pages to the lowest indices: up to max_moves moves for
+ * hl_kv_pages_copy, *n_moves of them, with the entries of the n_tables tables
+ * (rows of blocks_per_seq, one after another) changed to match.  A page that
+ * other tables hold too stays.  Afterwards upload the tables and run the copy
+ * before the next use.                                                      */
+int hl_page_pool_compact(hl_page_pool* pool, int32_t* tables, int n_tables, int blocks_per_seq, int32_t* moves,
+                         int max_moves, int* n_moves);
+
 #ifdef __cplusplus
 }
 #endif
