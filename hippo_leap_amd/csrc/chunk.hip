@@ -26,226 +26,60 @@
 
 namespace hl {
 
-struct ChunkParams {
-  ChunkSeqs s;
-  const void* q;
-  const void* k;
-  const void* v;
-  void* out;
-  unsigned* slots;
-  float* ws_o;   // [unit][split][rows][D]: sums of p * v
-  float* ws_ml;  // [unit][split][rows][2]: running max (log2 units), sum of p
-  int64_t q_stride, out_stride;
-  int col, io_dtype;
-  int n_head, group, window, n_sink;
-  int direct;    // work item = sequence (each chunk fits one row block)
-  int tps;       // 32-key tiles per split
-  int splits;    // most splits of a unit
-  float scale_log2;
-};
-
 namespace {
-typedef __attribute__((address_space(3))) void lds_void_t;
-typedef __attribute__((address_space(1))) const void global_cvoid_t;
-typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-
-// The operand type of the matrix products: the caches' type, fp16 for fp8
-// (which it holds exactly).
-template <int KVT>
-struct OpT;
-template <>
-struct OpT<HL_F16> {
-  static constexpr int dt = HL_F16;
-  static constexpr uint16_t exp_mask = 0x7C00;
-  typedef f16x8 vec;
-  static __device__ __forceinline__ f32x4 mma(u16x8 a, u16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
-  }
-};
-template <>
-struct OpT<HL_FP8> : OpT<HL_F16> {};
-template <>
-struct OpT<HL_BF16> {
-  static constexpr int dt = HL_BF16;
-  static constexpr uint16_t exp_mask = 0x7F80;
-  typedef bf16x8 vec;
-  static __device__ __forceinline__ f32x4 mma(u16x8 a, u16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
-  }
-};
-
-// 16 bytes per lane from global memory to LDS at dst + 16 * lane (dst
-// uniform); vmcnt counts it.
-__device__ __forceinline__ void copy16_to_lds(const void* src, void* dst) {
-  __builtin_amdgcn_global_load_lds((global_cvoid_t*)src, (lds_void_t*)dst, 16, 0, 0);
-}
-
-// Transposing LDS read: lane 16q + i of a 16-lane group gives the address of
-// 4 elements; lane 16q + i gets element i % 4 of lanes 16q + 4j + i / 4 as
-// its element j.  With lane 4j + a at row j, columns 4a .. 4a + 3 of a
-// 4 x 16 block, lane i ends up with column i's 4 rows.
-__device__ __forceinline__ i16x4 read_tr(const uint16_t* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)p);
-}
-
-// At most n of this wave's vector memory operations outstanding (in order).
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0F70);
-  asm volatile("" ::: "memory");
-}
-__device__ __forceinline__ void wait_lgkm() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-  asm volatile("" ::: "memory");
-}
-
-__device__ __forceinline__ bool sees(const ChunkParams& p, int j, int pos) {
-  return j <= pos && (p.window == 0 || pos - j < p.window || j < p.n_sink);
-}
-
-// The 32-key tiles that rows at positions p_lo .. p_hi read: the sinks', then
-// those from the first row's window to the last row.
-struct ChunkTiles {
-  int first, sinks, n;
-  __device__ __forceinline__ int at(int i) const { return i < sinks ? i : first + i - sinks; }
-};
-__device__ __forceinline__ ChunkTiles chunk_tiles(const ChunkParams& p, int p_lo, int p_hi) {
-  ChunkTiles t;
-  const int lo = p.window ? max(0, p_lo - p.window + 1) : 0;
-  t.first = lo >> 5;
-  t.sinks = p.window ? min((int)(((unsigned)p.n_sink + 31u) >> 5), t.first) : 0;
-  t.n = p_hi < 0 ? 0 : t.sinks + (p_hi >> 5) - t.first + 1;
-  return t;
-}
-
-// x (fp32) as the sum of N values of the operand type, the largest first.
-template <int DT, int N>
-__device__ __forceinline__ void split_parts(const float* x, u16x8* part) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float r = x[e];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint16_t b = to_bits<DT>(r);
-      part[i][e] = b;
-      if (i + 1 < N) r -= from_bits<DT>(b);
-    }
-  }
-}
-
-// Row r of a (sequence, kv head): element d of its query head's activation.
-__device__ __forceinline__ int64_t row_off(const ChunkParams& p, const ChunkSeq& c, int kvh, int r, int D, int d,
-                                           int64_t stride) {
-  const int t = r / p.group, h = kvh * p.group + (r - t * p.group);
-  return act_off(p.col, stride, h * D + d, c.lo + t);
-}
-
-// One row over tiles i0, i0 + step .. < i1 in plain fp32 arithmetic: what a
-// wave falls back to where an inf or NaN of V must reach some rows of its
-// block and not others (in the matrix product 0 * inf would).  Scores: lane
-// l has key l % 32 and half the dims; sums: dims l + 64e.
-template <int D, int KVT>
-__device__ void plain_row(const ChunkParams& p, const ChunkSeq& c, int b, int kvh, int r, ChunkTiles tl, int i0,
-                          int i1, int step, float& m, float& l, float* o) {
-  const int lane = threadIdx.x & 63, key = lane & 31, hh = lane >> 5;
-  constexpr int E = D / 64;
-  float q[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = act_load(p.q, p.io_dtype, row_off(p, c, kvh, r, D, lane + 64 * e, p.q_stride)) * p.scale_log2;
-    o[e] = 0.f;
-  }
-  m = -INFINITY;
-  l = 0.f;
-  const int pos = c.pos0 + r / p.group;
-  for (int i = i0; i < i1; i += step) {
-    const int t = tl.at(i), page = chunk_page(p.s, b, t);
-    if (page < 0) continue;
-    const int64_t base = ((int64_t)page * p.s.n_head_kv + kvh) * (D * 32);
-    float s = 0.f;
-    for (int d = 0; d < D / 2; ++d) {
-      const int dd = hh * (D / 2) + d;
-      float qd = __shfl(q[0], dd & 63, 64);
-      if constexpr (E > 1) {
-        const float q1 = __shfl(q[E - 1], dd & 63, 64);
-        qd = dd < 64 ? qd : q1;
-      }
-      s += qd * load_elem<KVT>(p.k, base + dd * 32 + key);
-    }
-    s += __shfl_xor(s, 32, 64);
-    const bool seen = sees(p, 32 * t + key, pos);
-    s = seen ? s : -INFINITY;
-    const unsigned mask = (unsigned)__builtin_amdgcn_ballot_w64(seen);  // lanes 0 .. 31: the keys
-    const float mn = fmaxf(m, wave_max(s)), ref = mn == -INFINITY ? 0.f : mn;
-    const float alpha = fast_exp2(m - ref), w = fast_exp2(s - ref);
-    m = mn;
-    l = l * alpha + 0.5f * wave_sum(w);  // each key is in two lanes
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= alpha;
-    for (int j = 0; j < 32; ++j) {
-      if (!((mask >> j) & 1u)) continue;
-      const float wj = __shfl(w, j, 64);
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += wj * load_elem<KVT>(p.v, base + (lane + 64 * e) * 32 + j);
-    }
-  }
-}
-
-// Weight of a partial with running max m against the joint max M (1 where
-// both are -inf: an empty partial is zero, and a NaN stays one).
-__device__ __forceinline__ float merge_weight(float m, float M) { return m == M ? 1.f : fast_exp2(m - M); }
-
 // The 4 waves' states of nrows rows (LDS, pitch D + 4) joined, then the
 // splits': written out by the last workgroup of the unit to arrive.
 template <int D, int ROWS>
 __device__ void chunk_finish(const ChunkParams& p, const ChunkSeq& c, int kvh, int r0, int nrows, int unit,
                              int split, int nsplit, const float* sm_m, const float* sm_l, const float* sm_o) {
   const int tid = threadIdx.x;
-  auto write = [&](int row, int d, float o, float l) {
-    act_store(p.out, p.io_dtype, row_off(p, c, kvh, r0 + row, D, d, p.out_stride), l == 0.f ? 0.f : o / l);
+  auto write = [&](int row, int d, f32x4 o, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (l == 0.f) o = f32x4{0.f, 0.f, 0.f, 0.f};
+    out_store4(p, row_off(p, c, kvh, r0 + row, D, d, p.out_stride), o * inv);
   };
   const int64_t at = ((int64_t)unit * p.splits + split) * ROWS;
-  for (int idx = tid; idx < nrows * D; idx += 256) {
-    const int row = idx / D, d = idx % D;
+  for (int idx = tid; idx < nrows * (D / 4); idx += 256) {
+    const int row = idx / (D / 4), d = idx % (D / 4) * 4;
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w * ROWS + row]);
-    float o = 0.f, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float f = merge_weight(sm_m[w * ROWS + row], M);
-      o += f * sm_o[(w * ROWS + row) * (D + 4) + d];
+      o += f * *(const f32x4*)&sm_o[(w * ROWS + row) * (D + 4) + d];
       l += f * sm_l[w * ROWS + row];
     }
     if (nsplit == 1) {
       write(row, d, o, l);
     } else {
-      store_agent(&p.ws_o[(at + row) * D + d], o);
-      if (d == 0) {
-        store_agent(&p.ws_ml[(at + row) * 2], M);
-        store_agent(&p.ws_ml[(at + row) * 2 + 1], l);
-      }
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) store_pair(&p.ws_o[(at + row) * D + d + e], o[e], o[e + 1]);
+      if (d == 0) store_pair(&p.ws_ml[(at + row) * 2], M, l);
     }
   }
   if (nsplit == 1) return;
   if (!arrive_last(&p.slots[unit], nsplit)) return;
-  for (int idx = tid; idx < nrows * D; idx += 256) {
-    const int row = idx / D, d = idx % D;
+  for (int idx = tid; idx < nrows * (D / 4); idx += 256) {
+    const int row = idx / (D / 4), d = idx % (D / 4) * 4;
     const float* ml = p.ws_ml + ((int64_t)unit * p.splits * ROWS + row) * 2;
     const float* wo = p.ws_o + ((int64_t)unit * p.splits * ROWS + row) * D + d;
-    float M = -INFINITY, l = 0.f, o = 0.f;
+    float M = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
     constexpr int U = 8;  // splits a memory round trip
     for (int s0 = 0; s0 < nsplit; s0 += U) {
-      float pm[U], pl[U], po[U];
+      float pm[U], pl[U];
+      f32x4 po[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t sp = min(s0 + u, nsplit - 1);
-        pm[u] = load_agent(&ml[sp * ROWS * 2]);
-        pl[u] = load_agent(&ml[sp * ROWS * 2 + 1]);
-        po[u] = load_agent(&wo[sp * ROWS * D]);
+        load_pair(&ml[sp * ROWS * 2], pm[u], pl[u]);
+        float x[4];
+        load_pair(&wo[sp * ROWS * D], x[0], x[1]);
+        load_pair(&wo[sp * ROWS * D + 2], x[2], x[3]);
+        po[u] = f32x4{x[0], x[1], x[2], x[3]};
       }
       float mn = M;
 #pragma unroll
@@ -270,8 +104,8 @@ __device__ void chunk_finish(const ChunkParams& p, const ChunkSeq& c, int kvh, i
 
 }  // namespace
 
-// Few rows: a workgroup takes one block of up to 16 * RB rows of one kv head
-// and a share of its key tiles, dealt to its 4 waves; every wave holds all
+// Few rows: a workgroup takes all rows of a (sequence, kv head), up to
+// 16 * RB, and a share of the key tiles, dealt to its 4 waves; every wave holds all
 // the rows and joins the others at the end.
 //   S^T[key][row] on v_mfma_f32_16x16x32, keys of half mb in the order
 //   8 * (m / 4) + 4 * mb + m % 4 (m the product's row), so that lane 16g + c
@@ -297,12 +131,11 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
   const int kvh = blockIdx.y, G = p.group;
-  int b = blockIdx.x, blk = 0;
-  if (!p.direct && !chunk_find(p.s, blockIdx.x, [&](int T, int) { return (T * G + ROWS - 1) / ROWS; }, b, blk)) return;
+  const int b = blockIdx.x, r0 = 0;
   const ChunkSeq cs = chunk_seq(p.s, b);
-  const int r0 = blk * ROWS, nrows = min(ROWS, cs.T * G - r0);
-  if (nrows <= 0) return;
-  const int p_lo = cs.pos0 + r0 / G, p_hi = cs.pos0 + (r0 + nrows - 1) / G;
+  const int nrows = cs.T * G;
+  if (nrows == 0 || nrows > p.rows_max) return;
+  const int p_lo = cs.pos0, p_hi = cs.pos0 + cs.T - 1;
   const ChunkTiles tl = chunk_tiles(p, p_lo, p_hi);
   const int nsplit = min(max(1, (tl.n + p.tps - 1) / p.tps), p.splits), split = blockIdx.z;
   if (split >= nsplit) return;
@@ -374,11 +207,13 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
     const bool live = row < nrows;
     pos[rb] = live ? cs.pos0 + (r0 + row) / G : -1;
     float x[KS][8];
+    q_load<KS>(p, cs, kvh, r0 + min(row, nrows - 1), D, 8 * g, 32, x);
+    if (!live) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        x[ks][e] = live ? act_load(p.q, p.io_dtype, row_off(p, cs, kvh, r0 + row, D, 32 * ks + 8 * g + e, p.q_stride)) : 0.f;
+        for (int e = 0; e < 8; ++e) x[ks][e] = 0.f;
+    }
     coef[rb] = p.scale_log2;
     if constexpr (MT == HL_F16) {
       uint32_t top = 0;
@@ -396,7 +231,7 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
       coef[rb] = ldexpf(p.scale_log2, -sh);
     }
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) split_parts<MT, NQ>(x[ks], qf[rb][ks]);
+    for (int ks = 0; ks < KS; ++ks) split_parts<KVT, NQ>(x[ks], qf[rb][ks]);
   }
 
   f32x4 o[RB][NB];
@@ -444,7 +279,7 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
       for (int e = 0; e < 8; ++e) x[e] = s[rb][e >> 2][e & 3] * coef[rb];
       if (!full) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = there && sees(p, j0 + 8 * g + e, pos[rb]) ? x[e] : -INFINITY;
+        for (int e = 0; e < 8; ++e) x[e] = there & sees(p, j0 + 8 * g + e, pos[rb], window_from(p, pos[rb])) ? x[e] : -INFINITY;
       }
       float top = x[0];
 #pragma unroll
@@ -463,7 +298,7 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
       l_run[rb] = l_run[rb] * alpha + sum;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) o[rb][nb] *= alpha;
-      split_parts<MT, NP>(x, pf[rb]);
+      split_parts<KVT, NP>(x, pf[rb]);
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -473,7 +308,7 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = j0 + 8 * g + e;
-          vf[e] = there && sees(p, j, max(j, p_lo)) && j <= p_hi ? vf[e] : (uint16_t)0;
+          vf[e] = there & sees(p, j, p_hi, window_from(p, p_lo)) ? vf[e] : (uint16_t)0;
           poison |= (vf[e] & Op::exp_mask) == Op::exp_mask;
         }
       }
@@ -560,8 +395,6 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
 // Host side
 // ---------------------------------------------------------------------------
 namespace {
-typedef void (*ChunkFn)(ChunkParams);
-
 template <int D, int KVT, bool HIGH>
 ChunkFn few_rb(int rb) {
   return rb == 1 ? chunk_few_kernel<D, KVT, HIGH, 1> : chunk_few_kernel<D, KVT, HIGH, 2>;
@@ -572,43 +405,81 @@ ChunkFn few_d(int kv, bool high, int rb) {
   if (kv == HL_FP8) return high ? few_rb<D, HL_FP8, true>(rb) : few_rb<D, HL_FP8, false>(rb);
   return high ? few_rb<D, HL_BF16, true>(rb) : few_rb<D, HL_BF16, false>(rb);
 }
-ChunkFn few_kernel(const hl_attn_chunk_args* a, int rb) {
-  const int kv = a->seqs.kv_dtype;
-  // fp16 activations have more bits than a bf16 operand.
-  const bool high = a->io_dtype == HL_F32 || (a->io_dtype == HL_F16 && kv == HL_BF16);
-  return a->seqs.head_dim == 64 ? few_d<64>(kv, high, rb) : few_d<128>(kv, high, rb);
-}
 
-// 32-key tiles that a block of rows at most `span` positions wide may read.
-int most_tiles(const hl_attn_chunk_args* a, int span) {
+// 32-key tiles that a block of rows touching at most `tokens` tokens may read.
+long long most_tiles(const hl_attn_chunk_args* a, int tokens) {
   const long long all = ((long long)a->seqs.max_kv + 31) / 32;
-  if (!a->window) return (int)all;
-  const long long seen = ((long long)a->window + span + 30) / 32 + 1 + ((long long)a->n_sink + 31) / 32;
-  return (int)std::min(all, seen);
+  if (!a->window) return all;
+  const long long seen = ((long long)a->window + tokens + 30) / 32 + 1 + ((long long)a->n_sink + 31) / 32;
+  return std::min(all, seen);
 }
 }  // namespace
 
 void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
   const hl_chunk_batch& s = a->seqs;
   memset(plan, 0, sizeof(*plan));
-  const int G = a->n_head / s.n_head_kv;
-  const long long most_rows = (long long)s.max_new * G;
-  plan->rb = most_rows <= 16 ? 1 : 2;
-  plan->rows = 16 * plan->rb;
-  plan->direct = most_rows <= plan->rows;
-  const long long rows = (long long)s.n_tokens * G;
-  plan->items = plan->direct ? s.batch : (int)(rows / plan->rows + std::min<long long>(s.batch, s.n_tokens));
-  const int tiles = most_tiles(a, (plan->rows + G - 2) / G + 1);  // tokens a block of rows may touch
-  const long long units = (long long)plan->items * s.n_head_kv;
-  long long S = units > kChunkSlots ? 1 : std::max<long long>(1, 2 * cu_count() / units);
-  if (a->num_splits > 0 && units <= kChunkSlots) S = a->num_splits;
-  S = std::min<long long>({S, std::max(1, (tiles + 3) / 4), 64});
-  plan->tps = (int)(((tiles + S - 1) / S + 3) / 4 * 4);
-  if (plan->tps < 4) plan->tps = 4;
-  plan->splits = std::max(1, (tiles + plan->tps - 1) / plan->tps);
-  plan->ws_bytes = plan->splits > 1
-                       ? kChunkSlots * 4 + (size_t)units * plan->splits * plan->rows * (s.head_dim + 2) * 4
-                       : 0;
+  const int G = a->n_head / s.n_head_kv, D = s.head_dim;
+  // fp16 activations have more bits than a bf16 operand.
+  plan->high = a->io_dtype == HL_F32 || (a->io_dtype == HL_F16 && s.kv_dtype == HL_BF16);
+  const long long most_rows = (long long)s.max_new * G, rows = (long long)s.n_tokens * G;
+
+  // Which kernel: chunks of up to 32 rows per kv head take the few-rows
+  // kernel, the others the flash kernel.  Where the longest chunk is longer,
+  // both run, and each takes the sequences that are its own: single tokens
+  // (16 rows, or 32 of larger groups) beside chunks.
+  const bool both = most_rows > 32;
+  plan->rb = (both ? G : most_rows) <= 16 ? 1 : 2;
+  plan->few.rows = 16 * plan->rb;
+  plan->few_max = both && G > 32 ? 0 : plan->few.rows;
+  if (plan->few_max > 0 && (!both || s.batch > 1)) plan->few.items = s.batch;
+  if (both) {
+    plan->tile.rows = plan->high ? 128 : 256;
+    const long long least = plan->few_max / G + 1;  // tokens of the shortest chunk it takes
+    plan->tile.items = (int)(rows / plan->tile.rows + std::min<long long>(s.batch, s.n_tokens / least));
+    if (plan->few.items == 0) plan->few_max = 0;
+    if (plan->tile.items == 0) plan->tile.items = 1;
+  }
+
+  plan->ws_bytes = 0;
+  size_t at = kChunkSlots * 4;
+  if (plan->few.items > 0) {
+    ChunkPart& f = plan->few;
+    const long long tiles = most_tiles(a, (f.rows + G - 2) / G + 1);
+    const long long units = (long long)f.items * s.n_head_kv;
+    long long S = units > kChunkSlots / 2 ? 1 : std::max<long long>(1, 2 * cu_count() / units);
+    if (a->num_splits > 0 && units <= kChunkSlots / 2) S = a->num_splits;
+    S = std::min<long long>({S, std::max<long long>(1, (tiles + 3) / 4), 64});
+    f.tps = (int)std::max<long long>(4, ((tiles + S - 1) / S + 3) / 4 * 4);
+    f.splits = (int)std::max<long long>(1, (tiles + f.tps - 1) / f.tps);
+    if (f.splits > 1) {
+      f.ws_at = at;
+      at += (size_t)units * f.splits * f.rows * (D + 2) * 4;
+      plan->ws_bytes = at;
+    }
+  }
+  if (plan->tile.items > 0) {
+    ChunkPart& t = plan->tile;
+    const long long tiles = (most_tiles(a, (t.rows + G - 2) / G + 1) + 1) / 2;
+    const long long units = (long long)t.items * s.n_head_kv;
+    const int waves = t.rows / 32;
+    // Workgroups run one per CU: the split count that needs the fewest rounds
+    // of tiles, each split costing about four more (its start and partials).
+    const int cus = cu_count();
+    long long best = 1, best_cost = 0;
+    const bool fits = units * waves <= kChunkSlots / 2;
+    for (long long S = 1; S <= (fits ? std::min<long long>(tiles, 32) : 1); ++S) {
+      const long long cost = (units * S + cus - 1) / cus * ((tiles + S - 1) / S + 4);
+      if (S == 1 || cost < best_cost) best = S, best_cost = cost;
+    }
+    if (a->num_splits > 0 && fits) best = std::min<long long>(a->num_splits, tiles);
+    t.tps = (int)((tiles + best - 1) / best);
+    t.splits = (int)((tiles + t.tps - 1) / t.tps);
+    if (t.splits > 1) {
+      t.ws_at = at;
+      at += (size_t)units * t.splits * t.rows * (D + 2) * 4;
+      plan->ws_bytes = at;
+    }
+  }
 }
 
 hipError_t chunk_attn_launch(const hl_attn_chunk_args* a, const ChunkAttnPlan* plan, void* ws, hipStream_t stream) {
@@ -628,21 +499,37 @@ hipError_t chunk_attn_launch(const hl_attn_chunk_args* a, const ChunkAttnPlan* p
   p.out_stride = a->out_stride ? a->out_stride : dense;
   p.col = col;
   p.io_dtype = a->io_dtype;
+  const int es = a->io_dtype == HL_F32 ? 4 : 2;
+  p.q_vec = !col && ((uintptr_t)a->q & 15) == 0 && p.q_stride * es % 16 == 0;
+  p.out_vec = !col && ((uintptr_t)a->out & (4 * es - 1)) == 0 && p.out_stride % 4 == 0;
   p.n_head = a->n_head;
   p.group = a->n_head / s.n_head_kv;
   p.window = a->window;
   p.n_sink = a->n_sink;
-  p.direct = plan->direct;
-  p.tps = plan->tps;
-  p.splits = plan->splits;
+  p.rows_min = plan->few_max + 1;
+  p.rows_max = plan->few_max;
   p.scale_log2 = (a->scale != 0.f ? a->scale : 1.0f / sqrtf((float)D)) * kLog2e;
-  if (ws) {
-    p.slots = (unsigned*)ws;
-    p.ws_o = (float*)((char*)ws + kChunkSlots * 4);
-    p.ws_ml = p.ws_o + (size_t)plan->items * s.n_head_kv * plan->splits * plan->rows * D;
+  // The flash kernel first: its workgroups are the longer ones.
+  for (int k = 0; k < 2; ++k) {
+    const ChunkPart& t = k == 0 ? plan->tile : plan->few;
+    if (t.items == 0) continue;
+    p.items = t.items;
+    p.tps = t.tps;
+    p.splits = t.splits;
+    if (t.splits > 1) {
+      p.slots = (unsigned*)ws + (k == 0 ? 0 : kChunkSlots / 2);
+      p.ws_o = (float*)((char*)ws + t.ws_at);
+      p.ws_ml = p.ws_o + (size_t)t.items * s.n_head_kv * t.splits * t.rows * D;
+    }
+    if (k == 0)
+      hipLaunchKernelGGL(chunk_tile_fn(D, s.kv_dtype, plan->high), dim3((unsigned)(t.items * t.splits) * s.n_head_kv),
+                         dim3(2 * t.rows), 0, stream, p);
+    else
+      hipLaunchKernelGGL(D == 64 ? few_d<64>(s.kv_dtype, plan->high, plan->rb) : few_d<128>(s.kv_dtype, plan->high, plan->rb),
+                         dim3(t.items, s.n_head_kv, t.splits), dim3(256), 0, stream, p);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(few_kernel(a, plan->rb), dim3(plan->items, s.n_head_kv, plan->splits), dim3(256), 0, stream, p);
-  return hipGetLastError();
+  return hipSuccess;
 }
 
 }  // namespace hl

@@ -261,11 +261,18 @@ bool linear_quant_norm_launch(int nmat, const void* const* w, float* const* y, c
 // ---- chunks of new tokens over paged caches --------------------------------
 // Attention (chunk.hip).  Workspace: kChunkSlots arrival counters, partials.
 constexpr int kChunkSlots = 4096;
+// One kernel's share of a call.
+struct ChunkPart {
+  int items;         // row blocks of all sequences, at most (0: not launched)
+  int rows;          // rows of a block
+  int tps, splits;   // key tiles per split, most splits of a row block
+  size_t ws_at;      // its partials in the workspace
+};
 struct ChunkAttnPlan {
-  int rb, rows;      // 16-row blocks, rows of a workgroup
-  bool direct;       // every chunk fits one workgroup's rows: work item = sequence
-  int items;         // row blocks of all sequences, at most
-  int tps, splits;   // 32-key tiles per split, most splits of a row block
+  bool high;         // products in fp32's precision
+  int rb;            // few: 16-row blocks of a workgroup
+  int few_max;       // rows of a (sequence, kv head) that the few-rows kernel takes
+  ChunkPart few, tile;
   size_t ws_bytes;
 };
 void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan);

@@ -20,6 +20,18 @@ __device__ __forceinline__ void store_agent(float* p, float v) {
 __device__ __forceinline__ float load_agent(const float* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// Two neighbouring floats (8-byte aligned) in one access.
+__device__ __forceinline__ void store_pair(float* p, float x, float y) {
+  __hip_atomic_store((unsigned long long*)p,
+                     (unsigned long long)__float_as_uint(x) | (unsigned long long)__float_as_uint(y) << 32,
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void load_pair(const float* p, float& x, float& y) {
+  const unsigned long long v =
+      __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  x = __uint_as_float((unsigned)v);
+  y = __uint_as_float((unsigned)(v >> 32));
+}
 __device__ __forceinline__ void wait_stores() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);  // no compiler reordering across
   __builtin_amdgcn_s_waitcnt(0x0F70);        // s_waitcnt vmcnt(0)
