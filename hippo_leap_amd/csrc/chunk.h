@@ -105,7 +105,6 @@ struct ChunkParams {
 };
 
 typedef __attribute__((address_space(3))) void lds_void_t;
-typedef __attribute__((address_space(1))) const void global_cvoid_t;
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 
@@ -142,10 +141,27 @@ struct OpT<HL_BF16> {
   }
 };
 
-// 16 bytes per lane from global memory to LDS at dst + 16 * lane (dst
-// uniform); vmcnt counts it.
-__device__ __forceinline__ void copy16_to_lds(const void* src, void* dst) {
-  __builtin_amdgcn_global_load_lds((global_cvoid_t*)src, (lds_void_t*)dst, 16, 0, 0);
+// 16 bytes per lane from global memory (uniform base, lane_bytes of the lane's
+// own) to LDS at byte lds_at + 16 * lane.  vmcnt counts it; it has no result
+// register.  Written out, because behind the builtin the compiler waits for
+// every copy in flight before any LDS read, whichever stage it reads (here a
+// stage's copies are waited for by count, wait_vm): 2048 tokens over 16K, head
+// dim 128, 566 -> 521 us; 16 sequences' single tokens 38.5 -> 35.4.
+__device__ __forceinline__ void copy16_to_lds(const void* base, unsigned lane_bytes, unsigned lds_at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds_at), "v"(lane_bytes), "s"((uint64_t)(uintptr_t)base)
+               : "memory", "m0");
+}
+// Byte address in LDS of a shared array's element.
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_void_t*)p);
+}
+
+// max of lanes l and l ^ 32.
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // Transposing LDS read: lane 16q + i of a 16-lane group gives the address of

@@ -154,6 +154,7 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
   const elem_t* kbase = (const elem_t*)p.k + (int64_t)kvh * TILE;
   const elem_t* vbase = (const elem_t*)p.v + (int64_t)kvh * TILE;
   uint16_t* const st0 = (uint16_t*)lds + wave * WAVE_ELEMS;  // [stage][K, V][D][32]
+  const unsigned lds_st0 = lds_address(st0);
 
   // LDS tiles: row d holds its four 16-byte chunks at chunk ^ ((d / 2) % 4),
   // so that the 16-byte reads of 8 neighbouring rows meet every bank once.
@@ -170,12 +171,13 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
 #pragma unroll
       for (int r = 0; r < CP; ++r) raw[1][r] = *(const u32x4*)(vs + r * 1024 + lane * 16);
     } else {
-      uint16_t* st = st0 + stage * 2 * TILE;
+      const unsigned st = lds_st0 + stage * 4 * TILE;
       const int row = lane >> 2, chunk = (lane & 3) ^ ((row >> 1) & 3);
+      const unsigned own = (row * 32 + 8 * chunk) * 2;
 #pragma unroll
-      for (int r = 0; r < CP; ++r) copy16_to_lds(ks + (16 * r + row) * 32 + 8 * chunk, st + r * 512);
+      for (int r = 0; r < CP; ++r) copy16_to_lds(ks + r * 512, own, st + r * 1024);
 #pragma unroll
-      for (int r = 0; r < CP; ++r) copy16_to_lds(vs + (16 * r + row) * 32 + 8 * chunk, st + TILE + r * 512);
+      for (int r = 0; r < CP; ++r) copy16_to_lds(vs + r * 512, own, st + 2 * TILE + r * 1024);
     }
   };
   // fp8: the loaded tile, converted, into the wave's one stage.

@@ -37,6 +37,10 @@ __device__ __forceinline__ int swz(int d) { return ((d >> 1) & 1) * 2 + ((d >> 2
 // a row's max exceeds it by this much (log2 units), so P <= 2^8.
 constexpr float kChunkRescale = 8.0f;
 
+__device__ __forceinline__ f32x16 zero16() {
+  return f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+}
+
 __device__ __forceinline__ void lds_barrier() {
   wait_lgkm();
   __builtin_amdgcn_s_barrier();
@@ -87,6 +91,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   const int i1 = split == nsplit - 1 ? nt : i0 + p.tps;
 
   const int n_tiles = i1 - i0;
+  bool missing = false;  // of the split's pages, one is not in the pool
 
   // The split's pages: the first ones in LDS, the others (contexts beyond
   // kChunkTilePages * 32 keys a split) looked up when they are needed.
@@ -100,7 +105,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   }
   auto page_at = [&](int j, int mb) {
     const int e = 2 * j + mb;
-    if (e < kChunkTilePages) return __builtin_amdgcn_readfirstlane(tab[e]);
+    if (e < kChunkTilePages) return tab[e];
     return 2 * i0 + e < tl.n ? chunk_page(p.s, b, tl.at(2 * i0 + e)) : -1;
   };
 
@@ -113,10 +118,20 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   const int pos = row_live ? cs.pos0 + row / G : -1;
   // First key of list entry 2j + mb (past the list's end: keys no row sees).
   auto key0 = [&](int j, int mb) { return 32 * tl.at(2 * (i0 + j) + mb); };
-  auto whole = [&](int j, int lo, int hi) {  // rows at lo .. hi see the whole tile
-    const int k0 = key0(j, 0), k1 = key0(j, 1);
-    return k1 + 31 <= lo && (p.window == 0 || ((hi - k0 < p.window || k0 + 31 < p.n_sink) &&
-                                               (hi - k1 < p.window || k1 + 31 < p.n_sink)));
+  // Tiles from .. to - 1 are seen whole by every row at positions lo .. hi:
+  // entries from e_lo on lie inside the last row's window, those before e_hi
+  // end at or before the first row.  (A tile of sinks counts as not whole.)
+  struct Whole {
+    int from, to;
+    __device__ __forceinline__ bool operator()(int j) const { return (j >= from) & (j < to); }
+  };
+  auto whole = [&](int lo, int hi) {
+    const int e_lo = p.window ? max(tl.sinks, tl.sinks + ((hi - p.window) >> 5) + 1 - tl.first) : 0;
+    const int e_hi = tl.sinks + ((lo + 1) >> 5) - tl.first;
+    Whole w;
+    w.from = ((e_lo + 1) >> 1) - i0;
+    w.to = missing ? w.from : (e_hi >> 1) - i0;
+    return w;
   };
 
   const int64_t page_elems = (int64_t)p.s.n_head_kv * PAGE;
@@ -128,18 +143,15 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
 
   // Tile j -> stage j % NS.  fp16 / bf16: direct copies, each wave its CP
   // blocks of 1 KB (16 rows of one page).
-  auto request = [&](const elem_t* base, uint16_t* st0, int j) {
+  const unsigned own = ((lane >> 2) * 32 + 8 * ((lane & 3) ^ swz(lane >> 2))) * 2;
+  const unsigned k_lds = lds_address(kst0) + wave * (CP * 1024), v_lds = lds_address(vst0) + wave * (CP * 1024);
+  const unsigned own_page = wave * CP / (D / 16), own_rows = wave * CP % (D / 16) * 1024;
+  auto request = [&](const elem_t* base, unsigned lds_at, int stage, int page) {
     if constexpr (KVT != HL_FP8) {
-      const int mb = wave * CP / (D / 16);
-      const int page = max(0, page_at(j, mb));
-      const uint16_t* src = base + page * page_elems;
-      uint16_t* st = st0 + (j % NS) * TILE;
+      // (the lookup is waited for here, not where it was made)
+      const char* src = (const char*)(base + max(0, __builtin_amdgcn_readfirstlane(page)) * page_elems) + own_rows;
 #pragma unroll
-      for (int r = 0; r < CP; ++r) {
-        const int blk1k = wave * CP + r;
-        const int d = (blk1k % (D / 16)) * 16 + (lane >> 2);
-        copy16_to_lds(src + d * 32 + 8 * ((lane & 3) ^ swz(d)), st + blk1k * 512);
-      }
+      for (int r = 0; r < CP; ++r) copy16_to_lds(src + r * 1024, own, lds_at + stage * (2 * TILE) + r * 1024);
     }
   };
   // fp8: 8 values per load, kept until the conversion into their stage.
@@ -150,7 +162,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
 #pragma unroll
       for (int r = 0; r < C8; ++r) {
         const int row8 = (r * W + wave) * 16;  // this wave's 16 rows of the tile
-        const int page = max(0, page_at(j, row8 / D));
+        const int page = max(0, __builtin_amdgcn_readfirstlane(page_at(j, row8 / D)));
         raw[r] = *(const u32x2v*)(base + page * page_elems + (row8 % D + (lane >> 2)) * 32 + 8 * (lane & 3));
       }
     }
@@ -201,8 +213,9 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
-  float m_ref = 0.f, l_run = 0.f;
-  bool any = false;  // the row has seen a key: m_ref is set
+  float m_ref = -INFINITY, l_run = 0.f;
+  float neg_ref = 0.f;  // -m_ref, 0 before the row's first key
+  Whole rows_whole, block_whole;
 
   // Fragment addresses.  K: lane 4j' + a of a 16-lane group reads row j',
   // columns of key group a of its 16 product rows (see read_tr); V: row ln.
@@ -227,7 +240,6 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
     return *(const u16x8*)(vst + (u >> 1) * PAGE + db * 1024 + voff[u & 1]);
   };
 
-  bool missing = false;  // of the split's pages, one is not in the pool
   // V columns of tile j that no row of the block sees to zero; notes an inf
   // or NaN among the rest.  `threads` threads from thread 0 on.
   auto clean_v = [&](int j, int threads) {
@@ -277,7 +289,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
       }
   };
   auto softmax = [&](int j) {
-    if (missing || !whole(j, w_lo, w_hi)) {
+    if (!rows_whole(j)) {
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb) {
         const int k0 = key0(j, mb);
@@ -294,14 +306,13 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[mb][i]);
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    mt *= coef;
-    const bool grew = any ? mt > m_ref + kChunkRescale : mt > -INFINITY;
+    mt = max_halves(mt) * coef;
+    const bool grew = mt > m_ref + kChunkRescale;
     if (__builtin_amdgcn_ballot_w64(grew) != 0) {  // uniform, rare after the first tiles
       const float mn = grew ? mt : m_ref;
-      const float alpha = any ? fast_exp2(m_ref - mn) : 1.f;  // nothing summed before the first
+      const float alpha = grew ? fast_exp2(m_ref - mn) : 1.f;  // 0 at the row's first key
       m_ref = mn;
-      any |= grew;
+      neg_ref = grew ? -mn : neg_ref;
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
@@ -316,7 +327,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = fast_exp2(fmaf(s[mb][8 * u + e], coef, -m_ref));
+          x[e] = fast_exp2(fmaf(s[mb][8 * u + e], coef, neg_ref));
           ps[e & 3] += x[e];
         }
         split_parts<KVT, NP>(x, pf[2 * mb + u]);
@@ -326,6 +337,8 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
 
   __syncthreads();
   missing = s_flags[0] != 0;
+  rows_whole = whole(w_lo, w_hi);
+  block_whole = whole(p_lo, p_hi);
   int wave_tiles = live ? n_tiles : 0;  // up to the wave's last position
   while (wave_tiles > 0 && key0(wave_tiles - 1, 0) > w_hi) --wave_tiles;
   if constexpr (HIGH) {
@@ -336,12 +349,13 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
         place8(kst0, kraw, j);
         place8(vst0, vraw, j);
       } else {
-        request(kbase, kst0, j);
-        request(vbase, vst0, j);
+        const int page = page_at(j, own_page);
+        request(kbase, k_lds, j % NS, page);
+        request(vbase, v_lds, j % NS, page);
         wait_vm<0>();
       }
       lds_barrier();
-      if (missing || !whole(j, p_lo, p_hi)) {
+      if (!block_whole(j)) {
         clean_v(j, NT);
         lds_barrier();
       }
@@ -384,17 +398,13 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) kf[k][mb] = m >= 1 ? kpre[k][mb] : kfrag(kst, mb, k);
 #pragma unroll
-        for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[mb][i] = 0.f;
-#pragma unroll
         for (int k = 0; k < KSTEPS; ++k) {
           if (k + AHEAD < KSTEPS) {
 #pragma unroll
             for (int mb = 0; mb < 2; ++mb) kf[(k + AHEAD) % (AHEAD + 1)][mb] = kfrag(kst, mb, k + AHEAD);
           }
 #pragma unroll
-          for (int mb = 0; mb < 2; ++mb) s[mb] = Op::mma32(kf[k % (AHEAD + 1)][mb], qf[k][0], s[mb]);
+          for (int mb = 0; mb < 2; ++mb) s[mb] = Op::mma32(kf[k % (AHEAD + 1)][mb], qf[k][0], k == 0 ? zero16() : s[mb]);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -417,6 +427,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
     // by the second phase of iteration m + 1 (the K fragments read ahead,
     // the columns of V cleaned): a phase before that the wave waits for
     // all but this iteration's copies.
+    int ks = 2, vs = 1, k_page = -1, v_page = -1;  // of the next copies: stages, pages
     auto copies = [&](int m) {
       if constexpr (KVT == HL_FP8) {
         if (m + 2 < n_tiles) place8(kst0, kraw, m + 2);
@@ -425,8 +436,13 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
         if (m + 2 < n_tiles) load8(vbase, vraw, m + 2);
         __builtin_amdgcn_sched_barrier(0);
       } else {
-        if (m + 2 < n_tiles) request(kbase, kst0, m + 2);
-        if (m + 1 < n_tiles) request(vbase, vst0, m + 1);
+        // stages: K(m+2) and V(m+1), ks and vs, go round with m
+        if (m + 2 < n_tiles) request(kbase, k_lds, ks, k_page);
+        if (m + 1 < n_tiles) request(vbase, v_lds, vs, v_page);
+        v_page = k_page;
+        k_page = m + 3 < n_tiles ? page_at(m + 3, own_page) : -1;
+        vs = ks;
+        ks = ks == NS - 1 ? 0 : ks + 1;
       }
     };
     auto landed = [&](int m) {
@@ -449,9 +465,16 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
       if (n_tiles > 2) load8(kbase, kraw, 2);
       if (n_tiles > 1) load8(vbase, vraw, 1);
     } else {
-      if (n_tiles > 0) request(kbase, kst0, 0);
-      if (n_tiles > 1) request(kbase, kst0, 1);
-      if (n_tiles > 0) request(vbase, vst0, 0);
+      if (n_tiles > 0) {
+        const int page = page_at(0, own_page);
+        request(kbase, k_lds, 0, page);
+        request(vbase, v_lds, 0, page);
+      }
+      if (n_tiles > 1) {
+        v_page = page_at(1, own_page);
+        request(kbase, k_lds, 1, v_page);
+      }
+      if (n_tiles > 2) k_page = page_at(2, own_page);
       wait_vm<0>();
     }
     lds_barrier();
@@ -462,7 +485,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
         matrix_step(m);
         __builtin_amdgcn_s_setprio(0);
         landed(m);
-        if (m < n_tiles && (missing || !whole(m, p_lo, p_hi))) clean_v(m, 256);
+        if (m < n_tiles && !block_whole(m)) clean_v(m, 256);
         vector_step(m);
         lds_barrier();
       }
@@ -483,7 +506,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   // The row's sums, and where its values lie: o[db][i] of lane (ln, hh) is
   // dim 32db + 8 (i / 4) + 4hh + i % 4.
   float l = l_run + __shfl_xor(l_run, 32, 64);
-  float m = any ? m_ref : -INFINITY;
+  float m = m_ref;
   const bool poison = s_flags[1] != 0;
   const int unit = (item * p.s.n_head_kv + kvh) * W + wave;
   if (poison) {  // row by row through LDS (the tiles are done with), one wave's part each
