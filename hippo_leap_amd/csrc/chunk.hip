@@ -434,12 +434,14 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
   plan->few.rows = 16 * plan->rb;
   plan->few_max = both && G > 32 ? 0 : plan->few.rows;
   if (plan->few_max > 0 && (!both || s.batch > 1)) plan->few.items = s.batch;
+  int long_seqs = 0;  // sequences that the flash kernel takes, at least
   if (both) {
     plan->tile.rows = plan->high ? 128 : 256;
-    const long long least = plan->few_max / G + 1;  // tokens of the shortest chunk it takes
-    plan->tile.items = (int)(rows / plan->tile.rows + std::min<long long>(s.batch, s.n_tokens / least));
+    const int single = plan->few.items ? plan->few_max / G : 0;  // tokens of the longest chunk that it does not take
     if (plan->few.items == 0) plan->few_max = 0;
-    if (plan->tile.items == 0) plan->tile.items = 1;
+    const long long most = std::min<long long>(s.batch, s.n_tokens / (single + 1));
+    plan->tile.items = (int)std::max<long long>(1, (rows + most * (plan->tile.rows - 1)) / plan->tile.rows);
+    long_seqs = (int)std::max<long long>(1, (s.n_tokens - (long long)s.batch * single) / std::max(1, s.max_new - single));
   }
 
   plan->ws_bytes = 0;
@@ -448,10 +450,18 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
     ChunkPart& f = plan->few;
     const long long tiles = most_tiles(a, (f.rows + G - 2) / G + 1);
     const long long units = (long long)f.items * s.n_head_kv;
-    long long S = units > kChunkSlots / 2 ? 1 : std::max<long long>(1, 2 * cu_count() / units);
-    if (a->num_splits > 0 && units <= kChunkSlots / 2) S = a->num_splits;
-    S = std::min<long long>({S, std::max<long long>(1, (tiles + 3) / 4), 64});
-    f.tps = (int)std::max<long long>(4, ((tiles + S - 1) / S + 3) / 4 * 4);
+    // The split count whose rounds of resident workgroups (by their LDS: one
+    // per CU at head dim 128, two at 64 or with fp8's one stage) take the
+    // fewest tiles per wave, each round costing about two more.
+    const int resident = cu_count() * (D == 64 || s.kv_dtype == HL_FP8 ? 2 : 1);
+    const bool fits = units <= kChunkSlots / 2;
+    long long S = 1, best_cost = 0;
+    for (long long n = 1; n <= (fits ? std::min<long long>((tiles + 3) / 4, 64) : 1); ++n) {
+      const long long cost = (units * n + resident - 1) / resident * (((tiles + n - 1) / n + 3) / 4 + 2);
+      if (n == 1 || cost < best_cost) S = n, best_cost = cost;
+    }
+    if (a->num_splits > 0 && fits) S = std::min<long long>({a->num_splits, std::max<long long>(1, (tiles + 3) / 4), 64});
+    f.tps = (int)std::max<long long>(4, (tiles + S - 1) / S);
     f.splits = (int)std::max<long long>(1, (tiles + f.tps - 1) / f.tps);
     if (f.splits > 1) {
       f.ws_at = at;
@@ -464,13 +474,23 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
     const long long tiles = (most_tiles(a, (t.rows + G - 2) / G + 1) + 1) / 2;
     const long long units = (long long)t.items * s.n_head_kv;
     const int waves = t.rows / 32;
-    // Workgroups run one per CU: the split count that needs the fewest rounds
-    // of tiles, each split costing about four more (its start and partials).
+    // Workgroups run one per CU.  The row blocks that there will be, not those
+    // there may be, count: full ones, and half of one or at least one for each
+    // long chunk that max_new and n_tokens imply (workgroups without a block
+    // end at once).  One long chunk: its blocks are alike, and the split count
+    // that needs the fewest rounds of tiles is taken, each split costing about
+    // four more (its start and partials).  Several: their contexts differ, and
+    // the last workgroup to start should not be a long one: the work per CU
+    // and one split more.  At most 1536 blocks of partials are kept.
     const int cus = cu_count();
+    const long long likely =
+        s.n_head_kv * std::min<long long>(t.items, std::max(long_seqs, (int)(rows / t.rows) + (long_seqs + 1) / 2));
     long long best = 1, best_cost = 0;
     const bool fits = units * waves <= kChunkSlots / 2;
-    for (long long S = 1; S <= (fits ? std::min<long long>(tiles, 32) : 1); ++S) {
-      const long long cost = (units * S + cus - 1) / cus * ((tiles + S - 1) / S + 4);
+    const long long most = fits ? std::min<long long>({tiles, 32, std::max<long long>(1, 1536 / units)}) : 1;
+    for (long long S = 1; S <= most; ++S) {
+      const long long piece = (tiles + S - 1) / S + 4;
+      const long long cost = long_seqs == 1 ? (likely * S + cus - 1) / cus * piece * cus : likely * S * piece + piece * cus;
       if (S == 1 || cost < best_cost) best = S, best_cost = cost;
     }
     if (a->num_splits > 0 && fits) best = std::min<long long>(a->num_splits, tiles);

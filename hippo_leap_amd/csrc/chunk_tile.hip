@@ -63,6 +63,11 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   constexpr int CP = D / 8 / W;                          // 1 KB copies per wave and tile (K or V)
   constexpr int C8 = 64 * D / 8 / NT;                    // fp8: 8-byte loads per thread and tile
   __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * NS * TILE];
+  // fp8, where a wave's share of a tile is 1 KB (8 waves, head dim 128): the
+  // bytes of the next K and V tile, copied as they are, so that they wait in
+  // LDS and not in registers (10 spilled).  Each wave converts its own.
+  constexpr bool RAW = KVT == HL_FP8 && !HIGH && D == 128;
+  __shared__ __attribute__((aligned(16))) unsigned char raw_lds[RAW ? 2 * 64 * D : 16];
   __shared__ int tab[kChunkTilePages];
   __shared__ int s_flags[2];  // a missing page; an inf or NaN that some rows must not meet
 
@@ -154,11 +159,16 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
       for (int r = 0; r < CP; ++r) copy16_to_lds(src + r * 1024, own, lds_at + stage * (2 * TILE) + r * 1024);
     }
   };
-  // fp8: 8 values per load, kept until the conversion into their stage.
+  // fp8 through registers: 8 values per load, kept until the conversion into
+  // their stage.
   typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
-  u32x2v kraw[KVT == HL_FP8 ? C8 : 1], vraw[KVT == HL_FP8 ? C8 : 1];
+  u32x2v kraw[KVT == HL_FP8 && !RAW ? C8 : 1], vraw[KVT == HL_FP8 && !RAW ? C8 : 1];
+  const unsigned raw_at = lds_address(raw_lds) + wave * 1024;
   auto load8 = [&](const elem_t* base, u32x2v* raw, int j) {
-    if constexpr (KVT == HL_FP8) {
+    if constexpr (RAW) {
+      const int page = max(0, __builtin_amdgcn_readfirstlane(page_at(j, wave >> 2)));
+      copy16_to_lds(base + page * page_elems + (wave & 3) * 1024, lane * 16, raw_at + (raw == vraw ? 64 * D : 0));
+    } else if constexpr (KVT == HL_FP8) {
 #pragma unroll
       for (int r = 0; r < C8; ++r) {
         const int row8 = (r * W + wave) * 16;  // this wave's 16 rows of the tile
@@ -168,14 +178,26 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
     }
   };
   auto place8 = [&](uint16_t* st0, const u32x2v* raw, int j) {
-    if constexpr (KVT == HL_FP8) {
-      uint16_t* st = st0 + (j % NS) * TILE;
+    uint16_t* st = st0 + (j % NS) * TILE;
+    if constexpr (RAW) {
+      const u32x4 x = *(const u32x4*)(raw_lds + (raw == vraw ? 64 * D : 0) + wave * 1024 + lane * 16);
+      const int rowd = 32 * wave + (lane >> 1), ch = 2 * (lane & 1), sw = swz(rowd);
+      *(u16x8*)(st + rowd * 32 + 8 * (ch ^ sw)) = e4m3x8_to_f16x8(x[0], x[1]);
+      *(u16x8*)(st + rowd * 32 + 8 * ((ch + 1) ^ sw)) = e4m3x8_to_f16x8(x[2], x[3]);
+    } else if constexpr (KVT == HL_FP8) {
 #pragma unroll
       for (int r = 0; r < C8; ++r) {
         const int rowd = (r * W + wave) * 16 + (lane >> 2);
         *(u16x8*)(st + rowd * 32 + 8 * ((lane & 3) ^ swz(rowd))) = e4m3x8_to_f16x8(raw[r][0], raw[r][1]);
       }
     }
+  };
+  // Raw bytes of this wave there; and read, so that others may follow.
+  auto raw_landed = [&]() {
+    if constexpr (RAW) wait_vm<0>();
+  };
+  auto raw_free = [&]() {
+    if constexpr (RAW) wait_lgkm();
   };
 
   // Q^T operand: lane (ln, hh) holds dims 16k + 8hh .. + 7 of its row.
@@ -342,34 +364,44 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   int wave_tiles = live ? n_tiles : 0;  // up to the wave's last position
   while (wave_tiles > 0 && key0(wave_tiles - 1, 0) > w_hi) --wave_tiles;
   if constexpr (HIGH) {
-    for (int j = 0; j < n_tiles; ++j) {
+    // Two stages: tile j + 1 is on its way while tile j is computed.  The
+    // barrier tells that tile j is there and that tile j - 1, whose stage
+    // tile j + 1 takes, is done with.
+    auto fetch = [&](int j) {
       if constexpr (KVT == HL_FP8) {
         load8(kbase, kraw, j);
         load8(vbase, vraw, j);
+      } else {
+        const int page = page_at(j, own_page);
+        request(kbase, k_lds, j & 1, page);
+        request(vbase, v_lds, j & 1, page);
+      }
+    };
+    if (n_tiles > 0) fetch(0);
+    for (int j = 0; j < n_tiles; ++j) {
+      if constexpr (KVT == HL_FP8) {
         place8(kst0, kraw, j);
         place8(vst0, vraw, j);
       } else {
-        const int page = page_at(j, own_page);
-        request(kbase, k_lds, j % NS, page);
-        request(vbase, v_lds, j % NS, page);
         wait_vm<0>();
       }
       lds_barrier();
+      if (j + 1 < n_tiles) fetch(j + 1);
       if (!block_whole(j)) {
         clean_v(j, NT);
         lds_barrier();
       }
       if (j < wave_tiles) {
-        products_qk(kst0 + (j % NS) * TILE);
+        products_qk(kst0 + (j & 1) * TILE);
         softmax(j);
-        products_pv(vst0 + (j % NS) * TILE);
+        products_pv(vst0 + (j & 1) * TILE);
       }
-      lds_barrier();
     }
+    lds_barrier();
   } else {
     // K fragments are read AHEAD steps before their products, the first ones
     // at the end of the softmax before.
-    constexpr int AHEAD = KVT == HL_FP8 && D == 128 ? 1 : 2;
+    constexpr int AHEAD = D == 128 ? 1 : 2;
     u16x8 kpre[AHEAD][2];
     // P V of tile m - 1, then S^T of tile m.  The steps are fenced, so that few
     // fragments are live; the SIMD's other wave covers their latency.
@@ -430,8 +462,10 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
     int ks = 2, vs = 1, k_page = -1, v_page = -1;  // of the next copies: stages, pages
     auto copies = [&](int m) {
       if constexpr (KVT == HL_FP8) {
+        raw_landed();
         if (m + 2 < n_tiles) place8(kst0, kraw, m + 2);
         if (m + 1 < n_tiles) place8(vst0, vraw, m + 1);
+        raw_free();
         if (m + 3 < n_tiles) load8(kbase, kraw, m + 3);
         if (m + 2 < n_tiles) load8(vbase, vraw, m + 2);
         __builtin_amdgcn_sched_barrier(0);
@@ -456,11 +490,11 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
     if constexpr (KVT == HL_FP8) {
       for (int j = 0; j < min(2, n_tiles); ++j) {
         load8(kbase, kraw, j);
+        if (j == 0) load8(vbase, vraw, 0);
+        raw_landed();
         place8(kst0, kraw, j);
-      }
-      if (n_tiles > 0) {
-        load8(vbase, vraw, 0);
-        place8(vst0, vraw, 0);
+        if (j == 0) place8(vst0, vraw, 0);
+        raw_free();
       }
       if (n_tiles > 2) load8(kbase, kraw, 2);
       if (n_tiles > 1) load8(vbase, vraw, 1);
@@ -563,32 +597,55 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   old = __builtin_amdgcn_readfirstlane(old);
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   if (old != (unsigned)(nsplit - 1)) return;
+  // The maxima, 8 splits a memory round trip; then the sums, 4 splits and 32
+  // dims (8 runs of 4) a trip.
   float M = -INFINITY;
-  for (int sp = 0; sp < nsplit; ++sp) {
-    float pm, pl;
-    load_pair(ml_at(sp), pm, pl);
-    M = fmaxf(M, pm);
+  for (int s0 = 0; s0 < nsplit; s0 += 8) {
+    float pm[8], pl[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) load_pair(ml_at(min(s0 + u, nsplit - 1)), pm[u], pl[u]);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) M = fmaxf(M, pm[u]);
   }
-  l = 0.f;
+  const int64_t to = row_off(p, cs, kvh, min(row, r0 + nrows - 1), D, 4 * hh, p.out_stride);
+  const int64_t by = p.col ? 8 * p.out_stride : 8;
+  for (int c0 = 0; c0 < DB * 4; c0 += 8) {
+    f32x4 acc[8];
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
+    for (int c = 0; c < 8; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    l = 0.f;
+    for (int s0 = 0; s0 < nsplit; s0 += 4) {
+      float pm[4], pl[4], x[4][8][4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
-  for (int sp = 0; sp < nsplit; ++sp) {
-    float pm, pl, x[DB][16];
-    load_pair(ml_at(sp), pm, pl);
+      for (int u = 0; u < 4; ++u) {
+        const int sp = min(s0 + u, nsplit - 1);
+        const float* from = pair_at(sp, 0, 0) + c0 * 256;
+        load_pair(ml_at(sp), pm[u], pl[u]);
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+        for (int c = 0; c < 8; ++c) {
+          load_pair(from + c * 256, x[u][c][0], x[u][c][1]);
+          load_pair(from + c * 256 + 128, x[u][c][2], x[u][c][3]);
+        }
+      }
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) load_pair(pair_at(sp, db, i), x[db][i], x[db][i + 1]);
-    const float w = merge_weight(pm, M);
-    l += w * pl;
+      for (int u = 0; u < 4; ++u) {
+        if (s0 + u < nsplit) {
+          const float w = merge_weight(pm[u], M);
+          l += w * pl[u];
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+          for (int c = 0; c < 8; ++c)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[db][i] += w * x[db][i];
+            for (int e = 0; e < 4; ++e) acc[c][e] += w * x[u][c][e];
+        }
+      }
+    }
+    if (row_live) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        out_store4(p, to + (c0 + c) * by, l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[c] * inv);
+    }
   }
-  write(o, l);
   if (lane == 0) __hip_atomic_store(&p.slots[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 

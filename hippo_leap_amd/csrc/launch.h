@@ -260,7 +260,7 @@ bool linear_quant_norm_launch(int nmat, const void* const* w, float* const* y, c
 
 // ---- chunks of new tokens over paged caches --------------------------------
 // Attention (chunk.hip).  Workspace: kChunkSlots arrival counters, partials.
-constexpr int kChunkSlots = 4096;
+constexpr int kChunkSlots = 16384;
 // One kernel's share of a call.
 struct ChunkPart {
   int items;         // row blocks of all sequences, at most (0: not launched)

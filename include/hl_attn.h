@@ -800,7 +800,7 @@ typedef struct hl_attn_chunk_args {
 } hl_attn_chunk_args;
 
 /* Device workspace hl_attn_chunk needs for these args (0: none), 16-byte
- * aligned: 16 KB of arrival counters, then the partial results of contexts
+ * aligned: 64 KB of arrival counters, then the partial results of contexts
  * split over workgroups.  The counters must be zero before the first call
  * (hl_attn_decode_workspace_init on the fresh workspace); each call leaves
  * them zero, so chunk calls of any shape may follow one another on one

@@ -90,7 +90,7 @@ def test_attn_refusals(hl, kw, text):
 def test_attn_workspace(hl):
     a = _attn({"max_kv": 32000, "blocks_per_seq": 1000, "max_new": 1, "n_tokens": 2})
     need = hl.hl_attn_chunk_workspace_bytes(ctypes.byref(a))
-    assert need > 16384
+    assert need > 65536
     for ws, n, text in ((None, need, "workspace"), (FAKE, need - 1, "needed"), (FAKE + 8, need, "16-byte")):
         assert hl.hl_attn_chunk(ctypes.byref(a), ws, n, None) == _lib.HL_EINVAL
         assert text in hl.hl_last_error().decode()
