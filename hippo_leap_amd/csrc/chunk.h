@@ -70,6 +70,46 @@ __device__ __forceinline__ bool chunk_find(const ChunkSeqs& s, int item, Count c
   return false;
 }
 
+// The same counted from the last part: item 0 is the last sequence's last
+// part.  Up to 64 sequences (one load of the lists per lane, the sequence's
+// own from its lane) the lists are read once; -1: no such part.
+template <typename Count>
+__device__ __forceinline__ int chunk_find_last(const ChunkSeqs& s, int item, Count count, int& part, ChunkSeq& c) {
+  if (s.batch > 64) {
+    int total = 0, b = -1;
+    const int lane = threadIdx.x & 63;
+    for (int b0 = 0; b0 < s.batch; b0 += 64) {
+      int lo;
+      int n = b0 + lane < s.batch ? count(chunk_len(s, b0 + lane, lo)) : 0;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+      total += __builtin_amdgcn_readfirstlane(n);
+    }
+    if (item >= total || !chunk_find(s, total - 1 - item, [&](int T, int) { return count(T); }, b, part)) return -1;
+    c = chunk_seq(s, b);
+    return b;
+  }
+  const int lane = threadIdx.x & 63, at = min(lane, s.batch - 1);
+  int lo;
+  const int T = chunk_len(s, at, lo), L = min(max(s.kv_lens[at], 0), s.max_kv);
+  const int n = lane < s.batch ? count(T) : 0;
+  int upto = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += x;
+  }
+  const int want = __builtin_amdgcn_readlane(upto, 63) - 1 - item;
+  if (want < 0) return -1;
+  const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > want));
+  part = want - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
+  c.lo = __builtin_amdgcn_readlane(lo, l);
+  c.T = __builtin_amdgcn_readlane(T, l);
+  c.L = __builtin_amdgcn_readlane(L, l);
+  c.pos0 = c.L - c.T;
+  return l;
+}
+
 // Element (row r, token t) of activations.
 __device__ __forceinline__ int64_t act_off(bool col, int64_t stride, int r, int t) {
   return col ? (int64_t)r * stride + t : (int64_t)t * stride + r;

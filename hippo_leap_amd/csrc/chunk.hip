@@ -230,7 +230,7 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[ks][e] = ldexpf(x[ks][e], sh);
-      coef[rb] = ldexpf(p.scale_log2, -sh);
+      coef[rb] = fmaxf(ldexpf(p.scale_log2, -sh), 1.2e-38f);  // above zero: -inf stays -inf
     }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) split_parts<KVT, NQ>(x[ks], qf[rb][ks]);
@@ -530,7 +530,7 @@ hipError_t chunk_attn_launch(const hl_attn_chunk_args* a, const ChunkAttnPlan* p
   p.n_sink = a->n_sink;
   p.rows_min = plan->few_max + 1;
   p.rows_max = plan->few_max;
-  p.scale_log2 = (a->scale != 0.f ? a->scale : 1.0f / sqrtf((float)D)) * kLog2e;
+  p.scale_log2 = std::max((a->scale != 0.f ? a->scale : 1.0f / sqrtf((float)D)) * kLog2e, 1.2e-38f);
   // The flash kernel first: its workgroups are the longer ones.
   for (int k = 0; k < 2; ++k) {
     const ChunkPart& t = k == 0 ? plan->tile : plan->few;

@@ -77,15 +77,16 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   const int G = p.group;
 
   // The kv head varies fastest, so that the 8 XCDs' L2 each keep their heads'
-  // pages; the last row blocks (the longest) start first.
+  // pages; items count from the last row block (a sequence's longest).
   int id = blockIdx.x;
   const int kvh = id % p.s.n_head_kv;
   id /= p.s.n_head_kv;
-  const int item = p.items - 1 - id % p.items, split = id / p.items;
-  int b, blk;
-  auto blocks = [&](int T, int) { return T * G >= p.rows_min ? (T * G + ROWS - 1) / ROWS : 0; };
-  if (!chunk_find(p.s, item, blocks, b, blk)) return;
-  const ChunkSeq cs = chunk_seq(p.s, b);
+  const int item = id % p.items, split = id / p.items;
+  int blk;
+  ChunkSeq cs;
+  auto blocks = [&](int T) { return T * G >= p.rows_min ? (T * G + ROWS - 1) / ROWS : 0; };
+  const int b = chunk_find_last(p.s, item, blocks, blk, cs);
+  if (b < 0) return;
   const int r0 = blk * ROWS, nrows = min(ROWS, cs.T * G - r0);
   const int p_lo = cs.pos0 + r0 / G, p_hi = cs.pos0 + (r0 + nrows - 1) / G;
   const ChunkTiles tl = chunk_tiles(p, p_lo, p_hi);
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
       for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[k][e] = ldexpf(x[k][e], sh);
-      coef = ldexpf(p.scale_log2, -sh);
+      coef = fmaxf(ldexpf(p.scale_log2, -sh), 1.2e-38f);  // above zero: -inf stays -inf
     }
 #pragma unroll
     for (int k = 0; k < KSTEPS; ++k) split_parts<KVT, NQ>(x[k], qf[k]);
