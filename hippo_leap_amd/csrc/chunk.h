@@ -396,7 +396,6 @@ __device__ __forceinline__ float merge_weight(float m, float M) { return m == M 
 // The flash kernel (chunk_tile.hip): 256 rows (high: 128, fp32 precision) per
 // workgroup of 64 threads per 32 rows.
 typedef void (*ChunkFn)(ChunkParams);
-ChunkFn chunk_tile_fn(int head_dim, int kv_dtype, bool high);
-constexpr int kChunkTilePages = 4096;  // pages of a split that its table in LDS holds
+ChunkFn chunk_tile_fn(int head_dim, int kv_dtype, bool high, bool pp);
 
 }  // namespace hl

@@ -436,7 +436,9 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
   if (plan->few_max > 0 && (!both || s.batch > 1)) plan->few.items = s.batch;
   int long_seqs = 0;  // sequences that the flash kernel takes, at least
   if (both) {
-    plan->tile.rows = plan->high ? 128 : 256;
+    // The 8-wave form (chunk_tile.hip) where its row blocks fill the GPU.
+    plan->pp = !plan->high && D == 128 && rows / 256 * s.n_head_kv >= cu_count();
+    plan->tile.rows = plan->pp ? 256 : 128;
     const int single = plan->few.items ? plan->few_max / G : 0;  // tokens of the longest chunk that it does not take
     if (plan->few.items == 0) plan->few_max = 0;
     const long long most = std::min<long long>(s.batch, s.n_tokens / (single + 1));
@@ -474,7 +476,7 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
     const long long tiles = (most_tiles(a, (t.rows + G - 2) / G + 1) + 1) / 2;
     const long long units = (long long)t.items * s.n_head_kv;
     const int waves = t.rows / 32;
-    // Workgroups run one per CU.  The row blocks that there will be, not those
+    // Resident workgroups: one or two per CU.  The row blocks that there will be, not those
     // there may be, count: full ones, and half of one or at least one for each
     // long chunk that max_new and n_tokens imply (workgroups without a block
     // end at once).  One long chunk: its blocks are alike, and the split count
@@ -482,7 +484,7 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
     // four more (its start and partials).  Several: their contexts differ, and
     // the last workgroup to start should not be a long one: the work per CU
     // and one split more.  At most 1536 blocks of partials are kept.
-    const int cus = cu_count();
+    const int cus = cu_count() * (plan->pp || (plan->high && D == 128) ? 1 : 2);
     const long long likely =
         s.n_head_kv * std::min<long long>(t.items, std::max(long_seqs, (int)(rows / t.rows) + (long_seqs + 1) / 2));
     long long best = 1, best_cost = 0;
@@ -544,7 +546,7 @@ hipError_t chunk_attn_launch(const hl_attn_chunk_args* a, const ChunkAttnPlan* p
       p.ws_ml = p.ws_o + (size_t)t.items * s.n_head_kv * t.splits * t.rows * D;
     }
     if (k == 0)
-      hipLaunchKernelGGL(chunk_tile_fn(D, s.kv_dtype, plan->high), dim3((unsigned)(t.items * t.splits) * s.n_head_kv),
+      hipLaunchKernelGGL(chunk_tile_fn(D, s.kv_dtype, plan->high, plan->pp), dim3((unsigned)(t.items * t.splits) * s.n_head_kv),
                          dim3(2 * t.rows), 0, stream, p);
     else
       hipLaunchKernelGGL(D == 64 ? few_d<64>(s.kv_dtype, plan->high, plan->rb) : few_d<128>(s.kv_dtype, plan->high, plan->rb),

@@ -48,27 +48,37 @@ __device__ __forceinline__ void lds_barrier() {
 }
 }  // namespace
 
-// PP (ping-pong): 8 waves, two per SIMD, in two groups one phase apart: while
-// one issues its matrix products the other runs its softmax.  Otherwise 4
-// waves, one per SIMD, with the registers for q and P in parts (HIGH).
-template <int D, int KVT, bool HIGH>
-__global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParams p) {
+// Two forms, which the plan chooses from:
+//  4 waves, two workgroups per CU (one with fp32's precision at head dim 128,
+//    whose parts of q and P take the registers): a SIMD's two waves run
+//    independently and fill each other's waits.
+//  PP, 8 waves in two groups one phase apart: while one group issues its
+//    matrix products the other runs its softmax.  Each tile in LDS serves
+//    twice the rows, but a phase lasts as long as its slower half.
+// Both at head dim 128 (us, 4 waves / PP): 2048 bf16 tokens over 16K, 4 kv
+// heads 490 / 478, fp8 581 / 513, 512 tokens at 8K, 8 kv heads 82.1 / 83.5,
+// 8 sequences' 5 tokens over 2K, 4 kv heads 30.8 / 40.  At head dim 64 the
+// softmax bounds both, and PP's phases are its latency: 512 tokens at 8K 51.6
+// / 59.0.
+template <int D, int KVT, bool HIGH, bool PP>
+__global__ __launch_bounds__(PP ? 512 : 256, HIGH && D == 128 ? 1 : 2) void chunk_tile_kernel(ChunkParams p) {
   typedef OpT<KVT> Op;
   constexpr int MT = Op::dt;
-  constexpr int W = HIGH ? 4 : 8, NT = 64 * W, ROWS = 32 * W;
+  constexpr int W = PP ? 8 : 4, NT = 64 * W, ROWS = 32 * W;
   constexpr int NQ = HIGH ? (MT == HL_BF16 ? 3 : 2) : 1, NP = NQ;
   constexpr int KSTEPS = D / 16, DB = D / 32;
   constexpr int PAGE = D * 32, TILE = 2 * PAGE;          // elements
-  constexpr int NS = HIGH ? 2 : 3;
+  constexpr int NS = PP ? 3 : 2;
+  constexpr int TABLE = 2048;                            // pages of the split that the table in LDS holds
   constexpr int CP = D / 8 / W;                          // 1 KB copies per wave and tile (K or V)
   constexpr int C8 = 64 * D / 8 / NT;                    // fp8: 8-byte loads per thread and tile
   __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * NS * TILE];
   // fp8, where a wave's share of a tile is 1 KB (8 waves, head dim 128): the
   // bytes of the next K and V tile, copied as they are, so that they wait in
   // LDS and not in registers (10 spilled).  Each wave converts its own.
-  constexpr bool RAW = KVT == HL_FP8 && !HIGH && D == 128;
+  constexpr bool RAW = KVT == HL_FP8 && PP && D == 128;
   __shared__ __attribute__((aligned(16))) unsigned char raw_lds[RAW ? 2 * 64 * D : 16];
-  __shared__ int tab[kChunkTilePages];
+  __shared__ int tab[TABLE];
   __shared__ int s_flags[2];  // a missing page; an inf or NaN that some rows must not meet
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -100,18 +110,18 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   bool missing = false;  // of the split's pages, one is not in the pool
 
   // The split's pages: the first ones in LDS, the others (contexts beyond
-  // kChunkTilePages * 32 keys a split) looked up when they are needed.
+  // TABLE * 32 keys a split) looked up when they are needed.
   if (tid < 2) s_flags[tid] = 0;
   __syncthreads();
   for (int e = tid; e < 2 * n_tiles; e += NT) {
     const int i = 2 * i0 + e;
     const int page = i < tl.n ? chunk_page(p.s, b, tl.at(i)) : -1;
     if (i < tl.n && page < 0) s_flags[0] = 1;
-    if (e < kChunkTilePages) tab[e] = page;
+    if (e < TABLE) tab[e] = page;
   }
   auto page_at = [&](int j, int mb) {
     const int e = 2 * j + mb;
-    if (e < kChunkTilePages) return tab[e];
+    if (e < TABLE) return tab[e];
     return 2 * i0 + e < tl.n ? chunk_page(p.s, b, tl.at(2 * i0 + e)) : -1;
   };
 
@@ -364,7 +374,7 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
   block_whole = whole(p_lo, p_hi);
   int wave_tiles = live ? n_tiles : 0;  // up to the wave's last position
   while (wave_tiles > 0 && key0(wave_tiles - 1, 0) > w_hi) --wave_tiles;
-  if constexpr (HIGH) {
+  if constexpr (!PP) {
     // Two stages: tile j + 1 is on its way while tile j is computed.  The
     // barrier tells that tile j is there and that tile j - 1, whose stage
     // tile j + 1 takes, is done with.
@@ -651,16 +661,21 @@ __global__ __launch_bounds__(HIGH ? 256 : 512) void chunk_tile_kernel(ChunkParam
 }
 
 namespace {
+template <int D, int KVT>
+ChunkFn tile_kv(bool high, bool pp) {
+  if (high) return chunk_tile_kernel<D, KVT, true, false>;
+  if constexpr (D == 128)
+    if (pp) return chunk_tile_kernel<D, KVT, false, true>;
+  return chunk_tile_kernel<D, KVT, false, false>;
+}
 template <int D>
-ChunkFn tile_d(int kv, bool high) {
-  if (kv == HL_F16) return high ? chunk_tile_kernel<D, HL_F16, true> : chunk_tile_kernel<D, HL_F16, false>;
-  if (kv == HL_FP8) return high ? chunk_tile_kernel<D, HL_FP8, true> : chunk_tile_kernel<D, HL_FP8, false>;
-  return high ? chunk_tile_kernel<D, HL_BF16, true> : chunk_tile_kernel<D, HL_BF16, false>;
+ChunkFn tile_d(int kv, bool high, bool pp) {
+  return kv == HL_F16 ? tile_kv<D, HL_F16>(high, pp) : (kv == HL_FP8 ? tile_kv<D, HL_FP8>(high, pp) : tile_kv<D, HL_BF16>(high, pp));
 }
 }  // namespace
 
-ChunkFn chunk_tile_fn(int head_dim, int kv_dtype, bool high) {
-  return head_dim == 64 ? tile_d<64>(kv_dtype, high) : tile_d<128>(kv_dtype, high);
+ChunkFn chunk_tile_fn(int head_dim, int kv_dtype, bool high, bool pp) {
+  return head_dim == 64 ? tile_d<64>(kv_dtype, high, pp) : tile_d<128>(kv_dtype, high, pp);
 }
 
 }  // namespace hl

@@ -270,6 +270,7 @@ struct ChunkPart {
 };
 struct ChunkAttnPlan {
   bool high;         // products in fp32's precision
+  bool pp;           // flash kernel: 8 waves in two groups (otherwise 4)
   int rb;            // few: 16-row blocks of a workgroup
   int few_max;       // rows of a (sequence, kv head) that the few-rows kernel takes
   ChunkPart few, tile;
