@@ -42,72 +42,38 @@ __device__ __forceinline__ int chunk_page(const ChunkSeqs& s, int b, int t) {
   return (unsigned)page < (unsigned)s.n_pages ? page : -1;
 }
 
-// Work item -> (sequence, part of its chunk): count(T) parts per sequence in
-// order.  One wave's work, redone by every wave: a prefix sum over the
-// sequences, 64 at a time.  false: past the last part.
+// Work item -> (sequence, part of its chunk), counted from the last sequence's
+// last part (a sequence's longest rows come first); count(T, L) parts per
+// sequence.  One wave's work, redone by every wave: a prefix sum over the
+// sequences, 64 at a time from the last ones, each lane reading one's lists.
+// -1: there is no such part.
 template <typename Count>
-__device__ __forceinline__ bool chunk_find(const ChunkSeqs& s, int item, Count count, int& b, int& part) {
+__device__ __forceinline__ int chunk_find_last(const ChunkSeqs& s, int item, Count count, int& part, ChunkSeq& c) {
   const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int b0 = 0; b0 < s.batch; b0 += 64) {
+  for (int b0 = (s.batch - 1) & ~63; b0 >= 0; b0 -= 64) {
+    const int at = min(b0 + lane, s.batch - 1);
     int lo;
-    const int n = b0 + lane < s.batch ? count(chunk_len(s, b0 + lane, lo), b0 + lane) : 0;
+    const int T = chunk_len(s, at, lo), L = min(max(s.kv_lens[at], 0), s.max_kv);
+    const int n = b0 + lane < s.batch ? count(T, L) : 0;
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int x = __shfl_up(upto, o, 64);
       if (lane >= o) upto += x;
     }
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(base + upto > item);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      b = b0 + l;
-      part = __builtin_amdgcn_readfirstlane(item - base - (__shfl(upto, l, 64) - __shfl(n, l, 64)));
-      return true;
+    const int want = __builtin_amdgcn_readlane(upto, 63) - 1 - item;
+    if (want >= 0) {
+      const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > want));
+      part = want - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
+      c.lo = __builtin_amdgcn_readlane(lo, l);
+      c.T = __builtin_amdgcn_readlane(T, l);
+      c.L = __builtin_amdgcn_readlane(L, l);
+      c.pos0 = c.L - c.T;
+      return b0 + l;
     }
-    base += __builtin_amdgcn_readlane(upto, 63);
+    item = -1 - want;
   }
-  return false;
-}
-
-// The same counted from the last part: item 0 is the last sequence's last
-// part.  Up to 64 sequences (one load of the lists per lane, the sequence's
-// own from its lane) the lists are read once; -1: no such part.
-template <typename Count>
-__device__ __forceinline__ int chunk_find_last(const ChunkSeqs& s, int item, Count count, int& part, ChunkSeq& c) {
-  if (s.batch > 64) {
-    int total = 0, b = -1;
-    const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < s.batch; b0 += 64) {
-      int lo;
-      int n = b0 + lane < s.batch ? count(chunk_len(s, b0 + lane, lo)) : 0;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-      total += __builtin_amdgcn_readfirstlane(n);
-    }
-    if (item >= total || !chunk_find(s, total - 1 - item, [&](int T, int) { return count(T); }, b, part)) return -1;
-    c = chunk_seq(s, b);
-    return b;
-  }
-  const int lane = threadIdx.x & 63, at = min(lane, s.batch - 1);
-  int lo;
-  const int T = chunk_len(s, at, lo), L = min(max(s.kv_lens[at], 0), s.max_kv);
-  const int n = lane < s.batch ? count(T) : 0;
-  int upto = n;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(upto, o, 64);
-    if (lane >= o) upto += x;
-  }
-  const int want = __builtin_amdgcn_readlane(upto, 63) - 1 - item;
-  if (want < 0) return -1;
-  const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > want));
-  part = want - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
-  c.lo = __builtin_amdgcn_readlane(lo, l);
-  c.T = __builtin_amdgcn_readlane(T, l);
-  c.L = __builtin_amdgcn_readlane(L, l);
-  c.pos0 = c.L - c.T;
-  return l;
+  return -1;
 }
 
 // Element (row r, token t) of activations.

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(PP ? 512 : 256, HIGH && D == 128 ? 1 : 2) void chun
   const int item = id % p.items, split = id / p.items;
   int blk;
   ChunkSeq cs;
-  auto blocks = [&](int T) { return T * G >= p.rows_min ? (T * G + ROWS - 1) / ROWS : 0; };
+  auto blocks = [&](int T, int) { return T * G >= p.rows_min ? (T * G + ROWS - 1) / ROWS : 0; };
   const int b = chunk_find_last(p.s, item, blocks, blk, cs);
   if (b < 0) return;
   const int r0 = blk * ROWS, nrows = min(ROWS, cs.T * G - r0);
