@@ -62,42 +62,54 @@ __device__ void chunk_finish(const ChunkParams& p, const ChunkSeq& c, int kvh, i
   }
   if (nsplit == 1) return;
   if (!arrive_last(&p.slots[unit], nsplit)) return;
-  for (int idx = tid; idx < nrows * (D / 4); idx += 256) {
-    const int row = idx / (D / 4), d = idx % (D / 4) * 4;
-    const float* ml = p.ws_ml + ((int64_t)unit * p.splits * ROWS + row) * 2;
-    const float* wo = p.ws_o + ((int64_t)unit * p.splits * ROWS + row) * D + d;
-    float M = -INFINITY, l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    constexpr int U = 8;  // splits a memory round trip
-    for (int s0 = 0; s0 < nsplit; s0 += U) {
-      float pm[U], pl[U];
-      f32x4 po[U];
+  // Two of a thread's runs of 4 dims and 4 splits a memory round trip.
+  const int64_t split_o = ROWS * D, split_ml = ROWS * 2;
+  const float* wo = p.ws_o + (int64_t)unit * p.splits * split_o;
+  const float* wm = p.ws_ml + (int64_t)unit * p.splits * split_ml;
+  const int n_idx = nrows * (D / 4);
+  for (int idx = tid; idx < n_idx; idx += 512) {
+    float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    f32x4 o[2];
+    int at2[2];  // second run: the first again where there is none
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t sp = min(s0 + u, nsplit - 1);
-        load_pair(&ml[sp * ROWS * 2], pm[u], pl[u]);
-        float x[4];
-        load_pair(&wo[sp * ROWS * D], x[0], x[1]);
-        load_pair(&wo[sp * ROWS * D + 2], x[2], x[3]);
-        po[u] = f32x4{x[0], x[1], x[2], x[3]};
-      }
-      float mn = M;
+    for (int i = 0; i < 2; ++i) {
+      at2[i] = i == 0 || idx + 256 < n_idx ? idx + 256 * i : idx;
+      o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int s0 = 0; s0 < nsplit; s0 += 4) {
+      float pm[2][4], pl[2][4], x[2][4][4];
 #pragma unroll
-      for (int u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
-      const float f = merge_weight(M, mn);
-      o *= f;
-      l *= f;
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (s0 + u < nsplit) {
-          const float w = merge_weight(pm[u], mn);
-          o += w * po[u];
-          l += w * pl[u];
+        for (int u = 0; u < 4; ++u) {
+          const int64_t sp = min(s0 + u, nsplit - 1);
+          const float* from = wo + sp * split_o + at2[i] * 4;
+          load_pair(wm + sp * split_ml + at2[i] / (D / 4) * 2, pm[i][u], pl[i][u]);
+          load_pair(from, x[i][u][0], x[i][u][1]);
+          load_pair(from + 2, x[i][u][2], x[i][u][3]);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mn = M[i];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mn = fmaxf(mn, pm[i][u]);
+        const float f = merge_weight(M[i], mn);
+        M[i] = mn;
+        o[i] *= f;
+        l[i] *= f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float w = s0 + u < nsplit ? merge_weight(pm[i][u], mn) : 0.f;
+          if (s0 + u < nsplit) {
+            l[i] += w * pl[i][u];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] += w * x[i][u][e];
+          }
         }
       }
-      M = mn;
     }
-    write(row, d, o, l);
+    write(at2[0] / (D / 4), at2[0] % (D / 4) * 4, o[0], l[0]);
+    if (idx + 256 < n_idx) write(at2[1] / (D / 4), at2[1] % (D / 4) * 4, o[1], l[1]);
   }
   if (tid == 0) __hip_atomic_store(&p.slots[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -194,6 +206,7 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
         }
     }
   };
+
   if (n_tiles > 0) {
     load_pages(0);
     request(0, 0);
@@ -203,18 +216,19 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
   u16x8 qf[RB][KS][NQ];
   float coef[RB];  // from a product to log2 units
   int pos[RB];
+  float x[RB][KS][8];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) q_load<KS>(p, cs, kvh, r0 + min(16 * rb + c, nrows - 1), D, 8 * g, 32, x[rb]);
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int row = 16 * rb + c;
     const bool live = row < nrows;
     pos[rb] = live ? cs.pos0 + (r0 + row) / G : -1;
-    float x[KS][8];
-    q_load<KS>(p, cs, kvh, r0 + min(row, nrows - 1), D, 8 * g, 32, x);
     if (!live) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[ks][e] = 0.f;
+        for (int e = 0; e < 8; ++e) x[rb][ks][e] = 0.f;
     }
     coef[rb] = p.scale_log2;
     if constexpr (MT == HL_F16) {
@@ -222,18 +236,18 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[ks][e]) & 0x7FFFFFFFu);
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[rb][ks][e]) & 0x7FFFFFFFu);
       top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
       top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
       const int sh = top >= kInfBits ? 0 : split_shift(top);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[ks][e] = ldexpf(x[ks][e], sh);
+        for (int e = 0; e < 8; ++e) x[rb][ks][e] = ldexpf(x[rb][ks][e], sh);
       coef[rb] = fmaxf(ldexpf(p.scale_log2, -sh), 1.2e-38f);  // above zero: -inf stays -inf
     }
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) split_parts<KVT, NQ>(x[ks], qf[rb][ks]);
+    for (int ks = 0; ks < KS; ++ks) split_parts<KVT, NQ>(x[rb][ks], qf[rb][ks]);
   }
 
   f32x4 o[RB][NB];
@@ -245,7 +259,11 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) o[rb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  bool poison = false;  // an inf or NaN of V that some rows must not meet
+  // Zero exponent bits, at least, of the V values that some rows must not meet
+  // (none: an inf or NaN).
+  u16x8 finite;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) finite[e] = 1;
 
   auto compute = [&](int n, int stage) {
     const int t = tl.at(i0 + 4 * n), j0 = 32 * t;
@@ -302,17 +320,19 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
       for (int nb = 0; nb < NB; ++nb) o[rb][nb] *= alpha;
       split_parts<KVT, NP>(x, pf[rb]);
     }
+    u16x8 some = {};  // keys that no row sees hold anything: their values to zero
+    if (!full) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        some[e] = there & sees(p, j0 + 8 * g + e, p_hi, window_from(p, p_lo)) ? (uint16_t)0xFFFF : (uint16_t)0;
+    }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int row = 16 * nb + c;
       u16x8 vf = *(const u16x8*)(vt + row * 32 + 8 * (g ^ ((row >> 1) & 3)));
-      if (!full) {  // keys that no row sees hold anything: zeros
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = j0 + 8 * g + e;
-          vf[e] = there & sees(p, j, p_hi, window_from(p, p_lo)) ? vf[e] : (uint16_t)0;
-          poison |= (vf[e] & Op::exp_mask) == Op::exp_mask;
-        }
+      if (!full) {
+        vf &= some;
+        finite = __builtin_elementwise_min(finite, (u16x8)(~vf & Op::exp_mask));
       }
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
@@ -362,6 +382,9 @@ __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
     l_run[rb] += __shfl_xor(l_run[rb], 32, 64);
   }
   __syncthreads();
+  bool poison = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) poison |= finite[e] == 0;
   float* sm_m = (float*)lds;
   float* sm_l = sm_m + 4 * ROWS;
   float* sm_o = sm_l + 4 * ROWS;
@@ -454,12 +477,17 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
     const long long units = (long long)f.items * s.n_head_kv;
     // The split count whose rounds of resident workgroups (by their LDS: one
     // per CU at head dim 128, two at 64 or with fp8's one stage) take the
-    // fewest tiles per wave, each round costing about two more.
+    // fewest tiles per wave, each round costing about two more and each memory
+    // round trip of the join (4 splits) one, at head dim 64 two of its smaller
+    // tiles.  8 sequences at 2K, head dim 64 (us by splits): 1 19.7, 2 13.9,
+    // 4 12.1, 8 12.9, 16 18.9; 16 windows of 4K, head dim 128: 2 33.9, 4 28.4,
+    // 8 33.2.
     const int resident = cu_count() * (D == 64 || s.kv_dtype == HL_FP8 ? 2 : 1);
     const bool fits = units <= kChunkSlots / 2;
     long long S = 1, best_cost = 0;
     for (long long n = 1; n <= (fits ? std::min<long long>((tiles + 3) / 4, 64) : 1); ++n) {
-      const long long cost = (units * n + resident - 1) / resident * (((tiles + n - 1) / n + 3) / 4 + 2);
+      const long long cost = (units * n + resident - 1) / resident * (((tiles + n - 1) / n + 3) / 4 + 2) +
+                             (n > 1 ? (n + 3) / 4 * (D == 64 ? 2 : 1) : 0);
       if (n == 1 || cost < best_cost) S = n, best_cost = cost;
     }
     if (a->num_splits > 0 && fits) S = std::min<long long>({a->num_splits, std::max<long long>(1, (tiles + 3) / 4), 64});
@@ -481,7 +509,9 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
     // long chunk that max_new and n_tokens imply (workgroups without a block
     // end at once).  One long chunk: its blocks are alike, and the split count
     // that needs the fewest rounds of tiles is taken, each split costing about
-    // four more (its start and partials).  Several: their contexts differ, and
+    // four more (its start) and a join eight (300 tokens at 300, head dim 128:
+    // unsplit 17.8 us, 2 splits 21; 512 at 8K: unsplit 153, 2 splits 93, 4 84, 8
+    // 93).  Several: their contexts differ, and
     // the last workgroup to start should not be a long one: the work per CU
     // and one split more.  At most 1536 blocks of partials are kept.
     const int cus = cu_count() * (plan->pp || (plan->high && D == 128) ? 1 : 2);
@@ -491,7 +521,7 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
     const bool fits = units * waves <= kChunkSlots / 2;
     const long long most = fits ? std::min<long long>({tiles, 32, std::max<long long>(1, 1536 / units)}) : 1;
     for (long long S = 1; S <= most; ++S) {
-      const long long piece = (tiles + S - 1) / S + 4;
+      const long long piece = (tiles + S - 1) / S + 4 + (S > 1 ? 8 : 0);
       const long long cost = long_seqs == 1 ? (likely * S + cus - 1) / cus * piece * cus : likely * S * piece + piece * cus;
       if (S == 1 || cost < best_cost) best = S, best_cost = cost;
     }

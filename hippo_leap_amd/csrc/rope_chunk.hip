@@ -92,13 +92,14 @@ __device__ __forceinline__ void act_store8(void* p, int64_t at, int64_t step, bo
 enum { kPairsHalf = 0, kPairsInterleaved = 1, kPairsAny = 2 };
 
 template <int D, int IO, int KVT, int PAIRS>
-__global__ __launch_bounds__(256, PAIRS == kPairsAny ? 2 : 4) void rope_chunk_kernel(RopeChunkParams p) {
+__global__ __launch_bounds__(256, PAIRS == kPairsAny ? 2 : (PAIRS == kPairsHalf && IO != HL_F32 && KVT == HL_F16 ? 3 : 4)) void rope_chunk_kernel(RopeChunkParams p) {
   constexpr int TPV = D / 16;       // threads of a head vector
   constexpr int VP = 256 / TPV;     // head vectors of a pass
   constexpr int TILES = VP / 32;    // whole-page tiles of a pass
   typedef typename std::conditional<KVT == HL_FP8, uint8_t, uint16_t>::type elem_t;
   __shared__ __attribute__((aligned(16))) elem_t tile[TILES * D * 32];
-  const int tid = threadIdx.x, k = tid & (TPV - 1), v = tid / TPV;
+  __shared__ float red[256];
+  const int tid = threadIdx.x;
 
   // The chunk's tokens in page block blk of sequence b.
   int part;
@@ -110,11 +111,16 @@ __global__ __launch_bounds__(256, PAIRS == kPairsAny ? 2 : 4) void rope_chunk_ke
   const int t0 = max(0, 32 * blk - cs.pos0), t1 = min(cs.T, 32 * blk + 32 - cs.pos0);
   const int ntok = t1 - t0, slot0 = (cs.pos0 + t0) & 31;
   const int page = blk >= 0 ? chunk_page(p.s, b, blk) : -1;
-  // Tokens to the next power of two: vector v is token v % n2 of head v / n2.
+  // Tokens to the next power of two, n2.  Threads run over a head vector's
+  // slots, then tokens, then heads where a token's dims are neighbours in
+  // memory; over tokens, slots, heads where a dim's tokens are.
   int lg = 0;
   while ((1 << lg) < ntok) ++lg;
-  const int n2 = 1 << lg, t = v & (n2 - 1), tok = cs.lo + t0 + min(t, ntok - 1);
-  const bool live = t < ntok;
+  const int n2 = 1 << lg;
+  const int k = p.col ? (tid >> lg) & (TPV - 1) : tid & (TPV - 1);
+  const int t = p.col ? tid & (n2 - 1) : (tid / TPV) & (n2 - 1), vh = tid / TPV >> lg;  // head of the pass
+  const int tok = cs.lo + t0 + min(t, ntok - 1);
+  const bool live = t < ntok, norm = p.q_norm_w || p.k_norm_w;
 
   // This thread's slots 8k .. 8k + 7: dims dim(e, 0) and dim(e, 1).  Half-split
   // with rope_dim % 16 == 0: two runs of 8 dims; interleaved: one of 16.
@@ -132,14 +138,18 @@ __global__ __launch_bounds__(256, PAIRS == kPairsAny ? 2 : 4) void rope_chunk_ke
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int s = 8 * k + e, i = min(s, max(half, 1) - 1);
-    sincospif(2.f * turn_of((float)(cs.pos0 + t0 + t), p.freqs.turns_hi[i], p.freqs.turns_lo[i]), &sv[e], &cv[e]);
+    // v_sin_f32 and v_cos_f32 take turns: off by 1.8e-7 at most over 16384
+    // positions, the angle's own error with it (sincospif: 3 to 6% slower).
+    const float turn = turn_of((float)(cs.pos0 + t0 + t), p.freqs.turns_hi[i], p.freqs.turns_lo[i]);
+    cv[e] = __builtin_amdgcn_cosf(turn);
+    sv[e] = __builtin_amdgcn_sinf(turn);
     cv[e] = s < half ? cv[e] * p.freqs.gain : 1.f;  // not rotated: as it is
     sv[e] = s < half ? sv[e] * p.freqs.gain : 0.f;
   }
   const int n_kv = p.s.n_head_kv, n_vec = p.n_head + 2 * n_kv;
   const int h_first = blockIdx.y * p.heads_wg, h_end = min(n_vec, h_first + p.heads_wg);
   for (int hp = h_first; hp < h_end; hp += VP >> lg) {
-    const int hv = hp + (v >> lg);
+    const int hv = hp + vh;
     const bool on = live && hv < h_end;
     const bool isq = hv < p.n_head, isk = !isq && hv < p.n_head + n_kv;
     const int h = isq ? hv : (isk ? hv - p.n_head : hv - p.n_head - n_kv);
@@ -168,18 +178,29 @@ __global__ __launch_bounds__(256, PAIRS == kPairsAny ? 2 : 4) void rope_chunk_ke
 #pragma unroll
       for (int e = 0; e < 8; ++e) x0[e] = x1[e] = 0.f;
     }
-    const float* w = isq ? p.q_norm_w : (isk ? p.k_norm_w : nullptr);
-    float ss = 0.f;
+    if (norm) {  // uniform
+      float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += x0[e] * x0[e] + x1[e] * x1[e];
+      for (int e = 0; e < 8; ++e) ss += x0[e] * x0[e] + x1[e] * x1[e];
+      if (p.col) {  // a vector's threads are n2 apart, in several waves
+        __syncthreads();
+        red[tid] = ss;
+        __syncthreads();
+        ss = 0.f;
 #pragma unroll
-    for (int o = 1; o < TPV; o <<= 1) ss += __shfl_xor(ss, o, 64);
-    if (w) {
-      const float inv = 1.0f / sqrtf(ss / (float)D + p.eps);
+        for (int i = 0; i < TPV; ++i) ss += red[((vh * TPV + i) << lg) + t];
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x0[e] *= inv * w[dim(e, 0)];
-        x1[e] *= inv * w[dim(e, 1)];
+        for (int o = 1; o < TPV; o <<= 1) ss += __shfl_xor(ss, o, 64);
+      }
+      const float* w = isq ? p.q_norm_w : (isk ? p.k_norm_w : nullptr);
+      if (w) {
+        const float inv = 1.0f / sqrtf(ss / (float)D + p.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x0[e] *= inv * w[dim(e, 0)];
+          x1[e] *= inv * w[dim(e, 1)];
+        }
       }
     }
     if (isq || isk) {
@@ -227,7 +248,7 @@ __global__ __launch_bounds__(256, PAIRS == kPairsAny ? 2 : 4) void rope_chunk_ke
       continue;
     }
     if (kv) {
-      elem_t* own = tile + (v >> 5) * (D * 32);
+      elem_t* own = tile + vh * (D * 32);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int d0 = dim(e, 0), d1 = dim(e, 1);
@@ -308,7 +329,8 @@ hipError_t rope_chunk_launch(const hl_rope_store_chunk_args* a, hipStream_t stre
   p.vec = !col && aligned(p.q, p.q_stride) && aligned(p.k, p.k_stride) && aligned(p.v, p.v_stride) &&
           aligned(p.q_out, p.q_out_stride);
   // Heads of a workgroup share its cos and sin; about 1024 workgroups cover
-  // the memory's latency.
+  // the memory's latency (2048 tokens, 48 head vectors: 512 19.6, 768 17.9,
+  // 1024 16.1, 2048 24.3 us).
   // Few tokens: a pass takes several heads, a quarter of a full one at least.
   int n2 = 1;
   while (n2 < 32 && n2 < s.max_new) n2 *= 2;
