@@ -441,15 +441,34 @@ def chunk_batch(k_pages, v_pages, block_table, q_start, kv_lens, n_tokens, max_n
     s.n_pages = k_pages.numel() // page
     s.k_pages, s.v_pages = _p(k_pages), _p(v_pages)
     s._tensors = (k_pages, v_pages, block_table, q_start, kv_lens)
+    s._device = _device_of(*s._tensors)
     return s
+
+
+def _device_of(*tensors):
+    """The one device of the tensors (None entries left out)."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise _lib.HLError(_lib.HL_EINVAL, f"the tensors lie on different devices: {sorted(map(str, devices))}")
+    return devices.pop().index
+
+
+def _on(device, stream):
+    """The stream's handle; HL_EINVAL where it, or the current device, is not the tensors'."""
+    current = torch.cuda.current_device()
+    at = current if stream is None else stream.device.index
+    if at != device or current != device:
+        raise _lib.HLError(_lib.HL_EINVAL, f"the tensors lie on cuda:{device}, the stream on cuda:{at}, "
+                                           f"the current device is cuda:{current}")
+    return _stream(stream)
 
 
 def _act(t, rows, n_tokens, layout, name):
     """(pointer, stride) of an activation tensor: [rows, n_tokens] column-major
     or [n_tokens, rows] token-major, its inner dimension contiguous."""
     want = (rows, n_tokens) if layout == HL_ACT_COLMAJOR else (n_tokens, rows)
-    if tuple(t.shape) != want or (want[1] > 1 and t.stride(1) != 1):
-        raise _lib.HLError(_lib.HL_EINVAL, f"{name} must be {want} with its last dimension contiguous")
+    if tuple(t.shape) != want or (want[1] > 1 and t.stride(1) != 1) or (want[0] > 1 and t.stride(0) < want[1]):
+        raise _lib.HLError(_lib.HL_EINVAL, f"{name} must be {want}, its rows apart and their elements neighbours")
     return _p(t), t.stride(0) if want[0] > 1 else 0
 
 
@@ -465,6 +484,7 @@ def attn_chunk_args(batch: ChunkBatch, q, out, n_head, act_layout=HL_ACT_COLMAJO
     a.out, a.out_stride = _act(out, rows, batch.n_tokens, act_layout, "out")
     a.scale, a.window, a.n_sink, a.num_splits = scale, window, n_sink, num_splits
     a._tensors = (batch, q, out)
+    a._device = _device_of(q, out, batch._tensors[0])
     return a
 
 
@@ -472,13 +492,13 @@ def attn_chunk_workspace_bytes(args: AttnChunkArgs) -> int:
     return int(_lib.load().hl_attn_chunk_workspace_bytes(ctypes.byref(args)))
 
 
-def attn_chunk_workspace(args: AttnChunkArgs, device="cuda", stream=None):
+def attn_chunk_workspace(args: AttnChunkArgs, stream=None):
     """Allocates and zero-initialises a workspace of hl_attn_chunk (None if not needed)."""
     nbytes = attn_chunk_workspace_bytes(args)
     if nbytes <= 0:
         return None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    check(_lib.load().hl_attn_decode_workspace_init(ws.data_ptr(), nbytes, _stream(stream)))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", args._device))
+    check(_lib.load().hl_attn_decode_workspace_init(ws.data_ptr(), nbytes, _on(args._device, stream)))
     return ws
 
 
@@ -486,7 +506,7 @@ def attn_chunk(args: AttnChunkArgs, workspace=None, stream=None) -> None:
     """hl_attn_chunk: attention of the chunk's tokens over their sequences' pages."""
     ws = workspace.data_ptr() if workspace is not None else None
     nbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    check(_lib.load().hl_attn_chunk(ctypes.byref(args), ws, nbytes, _stream(stream)))
+    check(_lib.load().hl_attn_chunk(ctypes.byref(args), ws, nbytes, _on(args._device, stream)))
 
 
 def rope_scaling(kind=HL_ROPE_SCALE_NONE, factor=1.0, original_len=0.0, low_freq=0.0, high_freq=0.0, beta_fast=0.0,
@@ -522,12 +542,13 @@ def rope_store_chunk_args(batch: ChunkBatch, q, k, v, q_out, n_head, rope_base, 
     a.q_norm_w, a.k_norm_w, a.eps, a.rope_style = _p(q_norm_w), _p(k_norm_w), eps, rope_style
     a.freqs = freqs if freqs is not None else rope_freqs(rope_dim or batch.head_dim, rope_base, scaling)
     a._tensors = (batch, q, k, v, q_out, q_norm_w, k_norm_w)
+    a._device = _device_of(q, k, v, q_out, q_norm_w, k_norm_w, batch._tensors[0])
     return a
 
 
 def rope_store_chunk(args: RopeStoreChunkArgs, stream=None) -> None:
     """hl_rope_store_chunk: qkNorm, rotation and the store into the pages."""
-    check(_lib.load().hl_rope_store_chunk(ctypes.byref(args), _stream(stream)))
+    check(_lib.load().hl_rope_store_chunk(ctypes.byref(args), _on(args._device, stream)))
 
 
 def kv_pages_args(pools) -> KvPages:
@@ -541,6 +562,7 @@ def kv_pages_args(pools) -> KvPages:
     a._pointers = (ctypes.c_void_p * len(pools))(*(_p(p) for p in pools))
     a.pools = ctypes.cast(a._pointers, ctypes.POINTER(ctypes.c_void_p))
     a._tensors = pools
+    a._device = _device_of(*pools)
     return a
 
 
@@ -549,7 +571,7 @@ def kv_pages_copy(args: KvPages, moves: torch.Tensor, stream=None) -> None:
     (from, to) of the host int32 tensor moves [n, 2]."""
     if moves.is_cuda or moves.dtype != torch.int32 or not moves.is_contiguous() or moves.numel() % 2:
         raise _lib.HLError(_lib.HL_EINVAL, "moves must be a contiguous int32 host tensor [n, 2]")
-    check(_lib.load().hl_kv_pages_copy(ctypes.byref(args), moves.data_ptr(), moves.numel() // 2, _stream(stream)))
+    check(_lib.load().hl_kv_pages_copy(ctypes.byref(args), moves.data_ptr(), moves.numel() // 2, _on(args._device, stream)))
 
 
 class PagePool:
@@ -602,6 +624,8 @@ class PagePool:
     def compact(self, tables, max_moves: int | None = None) -> torch.Tensor:
         """Moves pages to the lowest indices; tables [n, blocks] change to match.
         Returns the moves [n, 2] for kv_pages_copy."""
+        if tables.dim() != 2:
+            raise _lib.HLError(_lib.HL_EINVAL, "tables is [n, blocks]")
         moves = torch.empty(tables.numel() if max_moves is None else max_moves, 2, dtype=torch.int32)
         n = ctypes.c_int(0)
         check(_lib.load().hl_page_pool_compact(self._h, self._table(tables), tables.shape[0], tables.shape[1],

@@ -359,8 +359,8 @@ __device__ void plain_row(const ChunkParams& p, const ChunkSeq& c, int b, int kv
 // both are -inf: an empty partial is zero, and a NaN stays one).
 __device__ __forceinline__ float merge_weight(float m, float M) { return m == M ? 1.f : fast_exp2(m - M); }
 
-// The flash kernel (chunk_tile.hip): 256 rows (high: 128, fp32 precision) per
-// workgroup of 64 threads per 32 rows.
+// The flash kernel (chunk_tile.hip): 128 rows per workgroup of 4 waves, or 256
+// per workgroup of 8 (pp); high: fp32 precision.
 typedef void (*ChunkFn)(ChunkParams);
 ChunkFn chunk_tile_fn(int head_dim, int kv_dtype, bool high, bool pp);
 

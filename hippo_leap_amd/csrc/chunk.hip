@@ -431,10 +431,14 @@ ChunkFn few_d(int kv, bool high, int rb) {
   return high ? few_rb<D, HL_BF16, true>(rb) : few_rb<D, HL_BF16, false>(rb);
 }
 
+// A window that no position leaves is none (and pos - window then keeps to 32
+// bits at positions below zero).
+int window_of(const hl_attn_chunk_args* a) { return a->window < a->seqs.max_kv ? a->window : 0; }
+
 // 32-key tiles that a block of rows touching at most `tokens` tokens may read.
 long long most_tiles(const hl_attn_chunk_args* a, int tokens) {
   const long long all = ((long long)a->seqs.max_kv + 31) / 32;
-  if (!a->window) return all;
+  if (!window_of(a)) return all;
   const long long seen = ((long long)a->window + tokens + 30) / 32 + 1 + ((long long)a->n_sink + 31) / 32;
   return std::min(all, seen);
 }
@@ -525,7 +529,7 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
       const long long cost = long_seqs == 1 ? (likely * S + cus - 1) / cus * piece * cus : likely * S * piece + piece * cus;
       if (S == 1 || cost < best_cost) best = S, best_cost = cost;
     }
-    if (a->num_splits > 0 && fits) best = std::min<long long>(a->num_splits, tiles);
+    if (a->num_splits > 0 && fits) best = std::min<long long>({a->num_splits, tiles, 256});
     t.tps = (int)((tiles + best - 1) / best);
     t.splits = (int)((tiles + t.tps - 1) / t.tps);
     if (t.splits > 1) {
@@ -558,7 +562,7 @@ hipError_t chunk_attn_launch(const hl_attn_chunk_args* a, const ChunkAttnPlan* p
   p.out_vec = !col && ((uintptr_t)a->out & (4 * es - 1)) == 0 && p.out_stride % 4 == 0;
   p.n_head = a->n_head;
   p.group = a->n_head / s.n_head_kv;
-  p.window = a->window;
+  p.window = window_of(a);
   p.n_sink = a->n_sink;
   p.rows_min = plan->few_max + 1;
   p.rows_max = plan->few_max;

@@ -4,6 +4,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
 #include <new>
 #include <vector>
 
@@ -27,7 +28,7 @@ int check_batch(const hl_chunk_batch& s, int n_head, const char* who) {
   if (n_head % s.n_head_kv) return set_error(HL_EINVAL, "GQA requires head_count divisible by head_count_kv");
   if (s.head_dim != 64 && s.head_dim != 128)
     return set_error(HL_EUNSUPPORTED, "%s: head_dim %d not built (64 or 128)", who, s.head_dim);
-  if (n_head > 65535 || s.n_head_kv > 16384) return set_error(HL_EUNSUPPORTED, "%s: too many heads", who);
+  if (n_head > 16384) return set_error(HL_EUNSUPPORTED, "%s: more than 16384 heads", who);
   if (s.kv_dtype == HL_F32) return set_error(HL_EUNSUPPORTED, "%s: paged KV caches are fp16/bf16/fp8 only", who);
   if (s.kv_dtype != HL_F16 && s.kv_dtype != HL_BF16 && s.kv_dtype != HL_FP8)
     return set_error(HL_EINVAL, "%s: unknown kv_dtype %d", who, s.kv_dtype);
@@ -99,6 +100,9 @@ int check_attn_chunk(const hl_attn_chunk_args* a) {
   if (act_overlaps(q, out) || overlaps(a->seqs.k_pages, pb, a->out, out.bytes) ||
       overlaps(a->seqs.v_pages, pb, a->out, out.bytes))
     return set_error(HL_EINVAL, "%s: out overlaps q or the pages", who);
+  // A launch's grid: a workgroup per 128 rows of a kv head and per sequence.
+  if (((long long)a->seqs.n_tokens * a->n_head / 128 + (long long)a->seqs.batch * a->seqs.n_head_kv) * 256 >= 1ll << 32)
+    return set_error(HL_EUNSUPPORTED, "%s: %d tokens of %d heads in one call", who, a->seqs.n_tokens, a->n_head);
   if (!(a->scale >= 0.f) || !isfinite(a->scale)) return set_error(HL_EINVAL, "%s: scale must be finite and not negative", who);
   if (a->window < 0 || a->n_sink < 0 || a->num_splits < 0)
     return set_error(HL_EINVAL, "%s: window %d, n_sink %d and num_splits %d must not be negative", who, a->window, a->n_sink, a->num_splits);
@@ -234,6 +238,12 @@ int hl_kv_pages_copy(const hl_kv_pages* pg, const int32_t* moves, int n_moves, v
   // Every move runs at once: a page written twice, or written and read, would
   // end up with either content.
   try {
+    std::vector<uintptr_t> at(pg->n_pools);
+    for (int i = 0; i < pg->n_pools; ++i) at[i] = (uintptr_t)pg->pools[i];
+    std::sort(at.begin(), at.end());
+    for (int i = 1; i < pg->n_pools; ++i)
+      if (at[i] - at[i - 1] < pg->page_bytes * (size_t)pg->n_pages)
+        return set_error(HL_EINVAL, "%s: two pools overlap", who);
     std::vector<uint8_t> use((size_t)pg->n_pages, 0);  // 1: read, 2: written
     for (int m = 0; m < n_moves; ++m) {
       const int32_t from = moves[2 * (size_t)m], to = moves[2 * (size_t)m + 1];

@@ -42,6 +42,15 @@ CASES = {
     "mixed_window": ([1, 64, 1, 300], [4000, 2000, 50, 300], 16, 2, 128, "bf16", "bf16", 500, 5, False),
     "many": ([1, 2, 3] * 50, [40, 2, 77] * 50, 8, 2, 64, "bf16", "bf16", 0, 0, False),
     "big_chunk": ([1500], [2600], 8, 2, 128, "bf16", "bf16", 0, 0, False),
+    # windows that nothing leaves, tokens at positions below zero
+    "window_endless": ([40, 3, 1], [30, 90, 700], 8, 2, 64, "bf16", "bf16", 2**31 - 1, 2**31 - 1, False),
+    "window_endless_tiles": ([300], [200], 8, 2, 128, "f16", "f16", 2**31 - 1, 4, False),
+    "window_all_but_one": ([70, 2], [700, 641], 8, 2, 64, "bf16", "fp8", 699, 2**31 - 1, False),
+    # enough row blocks for the 8-wave form (head dim 128, 256 blocks of 256 rows)
+    "eight_waves": ([2048], [2300], 32, 8, 128, "bf16", "bf16", 0, 0, False),
+    "eight_waves_fp8": ([1700, 1, 500], [1700, 900, 2111], 32, 8, 128, "bf16", "fp8", 0, 0, False),
+    "eight_waves_f16_window": ([33, 2050, 0, 40], [4000, 2050, 100, 95], 32, 8, 128, "f16", "f16", 700, 40, True),
+    "eight_waves_nothing": ([2300], [1900], 32, 8, 128, "bf16", "bf16", 0, 0, False),
 }
 
 
@@ -155,14 +164,15 @@ def test_pages_outside_the_window_are_not_needed(hl, new, window):
 
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("which", ["k", "v"])
-@pytest.mark.parametrize("new,kv", [(3, "f16"), (50, "bf16"), (300, "bf16"), (300, "f16")])
-def test_not_finite_reaches_only_who_sees_it(hl, value, which, new, kv):
+@pytest.mark.parametrize("new,kv,heads,d", [(3, "f16", (8, 2), 64), (50, "bf16", (8, 2), 64), (300, "bf16", (8, 2), 64),
+                                            (300, "f16", (8, 2), 64), (2060, "bf16", (32, 8), 128)])
+def test_not_finite_reaches_only_who_sees_it(hl, value, which, new, kv, heads, d):
     """An inf or NaN at a new token's k or v, and at one that the window has
     left behind for some rows: the other rows keep their finite results."""
     from hippo_leap_amd import attention as A
     print(f"{which} {value} new {new}", flush=True)
     length, window = new + 70, 60
-    c = Case([new], [length], 8, 2, 64, "bf16", kv, seed=new)
+    c = Case([new], [length], *heads, d, "bf16", kv, seed=new)
     c.run_attn(A, window, 2)
     clean = c.tokens(c.out)
     marks = [length - 2, length - new - window + 2][:1 if new < 4 else 2]  # both would reach each of 3 rows
@@ -189,6 +199,31 @@ def test_not_finite_reaches_only_who_sees_it(hl, value, which, new, kv):
         assert torch.isfinite(rest).all()
     elif not (value == -math.inf or value == math.inf):
         assert torch.isnan(got[touched]).all()
+
+
+@pytest.mark.parametrize("new,io,kv", [(1, "f32", "f16"), (40, "bf16", "bf16"), (40, "f32", "fp8")])
+def test_contexts_beyond_the_page_table_in_lds(hl, new, io, kv):
+    """One workgroup walks more pages (2048 and more) than its table holds;
+    pages missing before and after that point."""
+    from hippo_leap_amd import attention as A
+    print(f"long {new} {io} {kv}", flush=True)
+    c = Case([new], [140001], 4, 1, 64, io, kv, seed=new)
+    c.table[0, 7] = -1
+    c.table[0, 4000] = c.n_pages
+    for splits in (1, 2, 0):
+        c.out.fill_(77)
+        c.run_attn(A, num_splits=splits)
+        check_attn(c, hidden_pages=(7, 4000))
+
+
+def test_missing_pages_in_the_eight_wave_form(hl):
+    from hippo_leap_amd import attention as A
+    for kv in ("bf16", "fp8"):
+        c = Case([2048], [2200], 32, 8, 128, "bf16", kv)
+        c.table[0, 3] = -1
+        c.table[0, 66] = c.n_pages + 1
+        c.run_attn(A, 1000, 4)
+        check_attn(c, window=1000, n_sink=4, hidden_pages=(3, 66))
 
 
 def test_offsets_past_32_bits(hl):

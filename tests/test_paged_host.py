@@ -58,6 +58,7 @@ BAD_BATCH = [
     ({"blocks_per_seq": 0}, _lib.HL_ECAPACITY, "blocks_per_seq"), ({"n_pages": 0}, _lib.HL_EINVAL, "n_pages"),
     ({"q_start": None}, _lib.HL_EINVAL, "null"), ({"kv_lens": None}, _lib.HL_EINVAL, "null"),
     ({"block_table": None}, _lib.HL_EINVAL, "null"), ({"block_table": FAKE + 2}, _lib.HL_EINVAL, "aligned"),
+    ({"n_head_kv": 16385}, _lib.HL_EINVAL, "divisible"),
     ({"k_pages": None}, _lib.HL_EINVAL, "pool"), ({"v_pages": (1 << 33) + 8}, _lib.HL_EINVAL, "16-byte"),
 ]
 
@@ -85,6 +86,15 @@ def test_attn_refusals(hl, kw, text):
     a = _attn(**kw)
     assert hl.hl_attn_chunk(ctypes.byref(a), FAKE, 1 << 40, None) == _lib.HL_EINVAL
     assert text in hl.hl_last_error().decode()
+
+
+def test_size_refusals(hl):
+    a = _attn({"n_tokens": 1 << 24, "max_new": 1 << 20}, n_head=128, q=1 << 40, out=1 << 44)
+    assert hl.hl_attn_chunk(ctypes.byref(a), FAKE, 1 << 40, None) == _lib.HL_EUNSUPPORTED
+    a = _attn({"n_head_kv": 1}, n_head=16385, q=1 << 40, out=1 << 44)
+    assert hl.hl_attn_chunk(ctypes.byref(a), FAKE, 1 << 40, None) == _lib.HL_EUNSUPPORTED
+    a = _attn({"n_tokens": (1 << 24) + 1})
+    assert hl.hl_attn_chunk(ctypes.byref(a), FAKE, 1 << 40, None) == _lib.HL_EUNSUPPORTED
 
 
 def test_attn_workspace(hl):
@@ -186,7 +196,8 @@ def test_copy_refusals(hl, moves, text):
 def test_copy_argument_refusals(hl):
     move = (ctypes.c_int32 * 2)(0, 1)
     for a, n in ((_pages(n_pools=0), 1), (_pages(n_pages=0), 1), (_pages(page_bytes=0), 1), (_pages(page_bytes=8), 1),
-                 (_pages(pools=(FAKE, None)), 1), (_pages(pools=(FAKE, FAKE + 8)), 1), (_pages(), -1)):
+                 (_pages(pools=(FAKE, None)), 1), (_pages(pools=(FAKE, FAKE + 8)), 1), (_pages(), -1),
+                 (_pages(pools=(FAKE, FAKE)), 1), (_pages(pools=(FAKE + 40944, FAKE)), 1)):
         assert hl.hl_kv_pages_copy(ctypes.byref(a), move, n, None) == _lib.HL_EINVAL
     assert hl.hl_kv_pages_copy(ctypes.byref(_pages()), None, 1, None) == _lib.HL_EINVAL
     assert hl.hl_kv_pages_copy(None, move, 1, None) == _lib.HL_EINVAL
@@ -321,3 +332,28 @@ def test_wrapper_refusals(hl):
         A.kv_pages_copy(_pages(), torch.zeros(1, 2))
     with pytest.raises(_lib.HLError):
         A.kv_pages_args([k, k[:2]])
+    x = torch.zeros(1, 128)
+    for t in (x.expand(4, 128), torch.zeros(128, 4).t(), torch.zeros(4, 64), torch.zeros(512)):
+        with pytest.raises(_lib.HLError):
+            A._act(t, 128, 4, _lib.HL_ACT_TOKENMAJOR, "q")
+
+
+def test_another_device_is_refused(hl, monkeypatch):
+    """Arguments made for one device, called with another one current or on
+    another one's stream: refused before the library is asked."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    a, r, p = _attn(), _rope(), _pages()
+    for args, call in ((a, A.attn_chunk), (r, A.rope_store_chunk),
+                       (p, lambda x, **kw: A.kv_pages_copy(x, torch.zeros(1, 2, dtype=torch.int32), **kw))):
+        args._device = 1
+        with pytest.raises(_lib.HLError) as e:
+            call(args)
+        assert "cuda:1" in str(e.value)
+
+    class Stream:
+        device = torch.device("cuda", 0)
+        cuda_stream = 0
+    with pytest.raises(_lib.HLError):
+        A.attn_chunk(a, stream=Stream())
+    with pytest.raises(_lib.HLError):
+        A._device_of(torch.zeros(1), torch.zeros(1, device="meta"))
