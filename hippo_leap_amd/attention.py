@@ -456,11 +456,10 @@ def _device_of(*tensors):
 def _on(device, stream):
     """The stream's handle; HL_EINVAL where it, or the current device, is not the tensors'."""
     current = torch.cuda.current_device()
-    at = current if stream is None else stream.device.index
-    if at != device or current != device:
-        raise _lib.HLError(_lib.HL_EINVAL, f"the tensors lie on cuda:{device}, the stream on cuda:{at}, "
-                                           f"the current device is cuda:{current}")
-    return _stream(stream)
+    if current != device or (stream is not None and stream.device.index != device):
+        raise _lib.HLError(_lib.HL_EINVAL, f"the tensors lie on cuda:{device}, the current device is cuda:{current}, "
+                                           f"the stream's {current if stream is None else stream.device}")
+    return _raw_stream(device) if stream is None and _raw_stream is not None else _stream(stream)
 
 
 def _act(t, rows, n_tokens, layout, name):
@@ -569,9 +568,10 @@ def kv_pages_args(pools) -> KvPages:
 def kv_pages_copy(args: KvPages, moves: torch.Tensor, stream=None) -> None:
     """hl_kv_pages_copy: page to becomes page from in every pool, for each row
     (from, to) of the host int32 tensor moves [n, 2]."""
-    if moves.is_cuda or moves.dtype != torch.int32 or not moves.is_contiguous() or moves.numel() % 2:
+    n = moves.numel()
+    if moves.is_cuda or moves.dtype != torch.int32 or not moves.is_contiguous() or n % 2:
         raise _lib.HLError(_lib.HL_EINVAL, "moves must be a contiguous int32 host tensor [n, 2]")
-    check(_lib.load().hl_kv_pages_copy(ctypes.byref(args), moves.data_ptr(), moves.numel() // 2, _on(args._device, stream)))
+    check(_lib.load().hl_kv_pages_copy(ctypes.byref(args), moves.data_ptr(), n // 2, _on(args._device, stream)))
 
 
 class PagePool:

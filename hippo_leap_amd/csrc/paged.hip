@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <functional>
 #include <new>
 #include <vector>
 
@@ -238,12 +239,16 @@ int hl_kv_pages_copy(const hl_kv_pages* pg, const int32_t* moves, int n_moves, v
   // Every move runs at once: a page written twice, or written and read, would
   // end up with either content.
   try {
-    std::vector<uintptr_t> at(pg->n_pools);
-    for (int i = 0; i < pg->n_pools; ++i) at[i] = (uintptr_t)pg->pools[i];
-    std::sort(at.begin(), at.end());
-    for (int i = 1; i < pg->n_pools; ++i)
-      if (at[i] - at[i - 1] < pg->page_bytes * (size_t)pg->n_pages)
-        return set_error(HL_EINVAL, "%s: two pools overlap", who);
+    const size_t bytes = pg->page_bytes * (size_t)pg->n_pages;
+    auto after = [&](const void* a, const void* b) { return (uintptr_t)b >= (uintptr_t)a + bytes; };
+    bool apart = true;
+    for (int i = 1; i < pg->n_pools; ++i) apart &= after(pg->pools[i - 1], pg->pools[i]);
+    if (!apart) {  // or not in ascending order
+      std::vector<const void*> at(pg->pools, pg->pools + pg->n_pools);
+      std::sort(at.begin(), at.end(), std::less<const void*>());
+      for (int i = 1; i < pg->n_pools; ++i)
+        if (!after(at[i - 1], at[i])) return set_error(HL_EINVAL, "%s: two pools overlap", who);
+    }
     std::vector<uint8_t> use((size_t)pg->n_pages, 0);  // 1: read, 2: written
     for (int m = 0; m < n_moves; ++m) {
       const int32_t from = moves[2 * (size_t)m], to = moves[2 * (size_t)m + 1];

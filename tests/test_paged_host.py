@@ -202,6 +202,10 @@ def test_copy_argument_refusals(hl):
     assert hl.hl_kv_pages_copy(ctypes.byref(_pages()), None, 1, None) == _lib.HL_EINVAL
     assert hl.hl_kv_pages_copy(None, move, 1, None) == _lib.HL_EINVAL
     assert hl.hl_kv_pages_copy(ctypes.byref(_pages()), None, 0, None) == _lib.HL_OK
+    # pools apart, in descending order: past that check (the move is what is refused)
+    bad = (ctypes.c_int32 * 2)(0, 10)
+    assert hl.hl_kv_pages_copy(ctypes.byref(_pages(pools=(FAKE + 40960, FAKE))), bad, 1, None) == _lib.HL_EINVAL
+    assert "outside" in hl.hl_last_error().decode()
 
 
 def _table(n):
