@@ -126,6 +126,10 @@ __device__ void chunk_finish(const ChunkParams& p, const ChunkSeq& c, int kvh, i
 // HIGH: fp32 activations, q and P in 3 bf16 (2 fp16) parts, which hold fp32's
 // bits (2 bf16 parts of P: 1.9e-6 off 64 bits at 4096 keys, 3: fp32's own
 // error).  A row's q is scaled by a power of two into fp16's range for fp16 operands.
+// Bound by HBM, and by latency where the keys are few: every wave keeps a tile
+// of its own in flight behind the one it computes, without barriers.  16
+// single tokens, head dim 128, fp32 on bf16: all of 32K 186 us (5.7 TB/s), a
+// window of 4096 32 us (4.2 TB/s); one token over 1024 keys 8.9 us.
 template <int D, int KVT, bool HIGH, int RB>
 __global__ __launch_bounds__(256) void chunk_few_kernel(ChunkParams p) {
   typedef OpT<KVT> Op;

@@ -57,7 +57,9 @@ __device__ __forceinline__ void lds_barrier() {
 //    twice the rows, but a phase lasts as long as its slower half.
 // Both at head dim 128 (us, 4 waves / PP): 2048 bf16 tokens over 16K, 4 kv
 // heads 490 / 478, fp8 581 / 513, 512 tokens at 8K, 8 kv heads 82.1 / 83.5,
-// 8 sequences' 5 tokens over 2K, 4 kv heads 30.8 / 40.  At head dim 64 the
+// 8 sequences' 5 tokens over 2K, 4 kv heads 30.8 / 40: 1.08 PFLOP/s, 980 and
+// 810 TFLOP/s at the first three.  Bound by the softmax's vector work beside
+// the products.  At head dim 64 the
 // softmax bounds both, and PP's phases are its latency: 512 tokens at 8K 51.6
 // / 59.0.
 template <int D, int KVT, bool HIGH, bool PP>

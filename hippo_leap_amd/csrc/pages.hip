@@ -24,7 +24,8 @@ struct PagesCopyParams {
 static_assert(sizeof(PagesCopyParams) <= 4096, "kernel arguments");
 
 // Workgroup (x, move, pool): 4 16-byte loads per thread in flight, 16 KB of
-// the page per workgroup.
+// the page per workgroup.  200 pages of 64 KB in 64 pools: 319 us, 5.26 TB/s; 3
+// pages in 32 pools 5.5 us, the launch.
 __global__ __launch_bounds__(256) void pages_copy_kernel(PagesCopyParams p) {
   const int m = blockIdx.y;
   char* pool = p.pool[blockIdx.z];
