@@ -24,9 +24,8 @@
 // block's rows are computed again, one by one, at the end.
 #include <cstring>
 
-#include "chunk.h"
+#include "chunk_few.h"
 #include "launch.h"
-#include "split_merge.h"
 
 namespace hl {
 
@@ -59,22 +58,26 @@ __device__ __forceinline__ void lds_barrier() {
 // heads 490 / 478, fp8 581 / 513, 512 tokens at 8K, 8 kv heads 82.1 / 83.5,
 // 8 sequences' 5 tokens over 2K, 4 kv heads 30.8 / 40: 1.08 PFLOP/s, 980 and
 // 810 TFLOP/s at the first three.  Bound by the softmax's vector work beside
-// the products.  At head dim 64 the
-// softmax bounds both, and PP's phases are its latency: 512 tokens at 8K 51.6
-// / 59.0.
+// the products.  At head dim 64 the softmax bounds both, and PP's phases are
+// its latency: 512 tokens at 8K 51.6 / 59.0.
+template <int D, bool PP>
+constexpr int kTileStages = PP ? 3 : 2;
+template <int D, bool PP>
+constexpr int kTileLds = 2 * kTileStages<D, PP> * 64 * D;  // elements
+
+// Workgroup `id` of the launch; lds: kTileLds elements, 1 KB aligned.
 template <int D, int KVT, bool HIGH, bool PP>
-__global__ __launch_bounds__(PP ? 512 : 256, HIGH && D == 128 ? 1 : 2) void chunk_tile_kernel(ChunkParams p) {
+__device__ __forceinline__ void chunk_tile(const ChunkParams& p, uint16_t* lds, int id) {
   typedef OpT<KVT> Op;
   constexpr int MT = Op::dt;
   constexpr int W = PP ? 8 : 4, NT = 64 * W, ROWS = 32 * W;
   constexpr int NQ = HIGH ? (MT == HL_BF16 ? 3 : 2) : 1, NP = NQ;
   constexpr int KSTEPS = D / 16, DB = D / 32;
   constexpr int PAGE = D * 32, TILE = 2 * PAGE;          // elements
-  constexpr int NS = PP ? 3 : 2;
+  constexpr int NS = kTileStages<D, PP>;
   constexpr int TABLE = 2048;                            // pages of the split that the table in LDS holds
   constexpr int CP = D / 8 / W;                          // 1 KB copies per wave and tile (K or V)
   constexpr int C8 = 64 * D / 8 / NT;                    // fp8: 8-byte loads per thread and tile
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * NS * TILE];
   // fp8, where a wave's share of a tile is 1 KB (8 waves, head dim 128): the
   // bytes of the next K and V tile, copied as they are, so that they wait in
   // LDS and not in registers (10 spilled).  Each wave converts its own.
@@ -90,7 +93,6 @@ __global__ __launch_bounds__(PP ? 512 : 256, HIGH && D == 128 ? 1 : 2) void chun
 
   // The kv head varies fastest, so that the 8 XCDs' L2 each keep their heads'
   // pages; items count from the last row block (a sequence's longest).
-  int id = blockIdx.x;
   const int kvh = id % p.s.n_head_kv;
   id /= p.s.n_head_kv;
   const int item = id % p.items, split = id / p.items;
@@ -662,6 +664,28 @@ __global__ __launch_bounds__(PP ? 512 : 256, HIGH && D == 128 ? 1 : 2) void chun
   if (lane == 0) __hip_atomic_store(&p.slots[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+template <int D, int KVT, bool HIGH, bool PP>
+__global__ __launch_bounds__(PP ? 512 : 256, HIGH && D == 128 ? 1 : 2) void chunk_tile_kernel(ChunkParams p) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[kTileLds<D, PP>];
+  chunk_tile<D, KVT, HIGH, PP>(p, lds, blockIdx.x);
+}
+
+// Both kernels' workgroups in one launch, the flash kernel's first.
+template <int D, int KVT, bool HIGH, int RB>
+__global__ __launch_bounds__(256, 2) void chunk_both_kernel(ChunkParams p, ChunkParams few, int n_tile) {
+  constexpr int A = kTileLds<D, false> * 2, B = ChunkFew<D, KVT, HIGH, RB>::LDS_BYTES;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[A > B ? A : B];
+  int id = blockIdx.x;
+  if (id < n_tile) {
+    chunk_tile<D, KVT, HIGH, false>(p, (uint16_t*)lds, id);
+    return;
+  }
+  id -= n_tile;
+  const int b = id % few.items;
+  id /= few.items;
+  chunk_few<D, KVT, HIGH, RB>(few, lds, b, id % few.s.n_head_kv, id / few.s.n_head_kv);
+}
+
 namespace {
 template <int D, int KVT>
 ChunkFn tile_kv(bool high, bool pp) {
@@ -675,6 +699,17 @@ ChunkFn tile_d(int kv, bool high, bool pp) {
   return kv == HL_F16 ? tile_kv<D, HL_F16>(high, pp) : (kv == HL_FP8 ? tile_kv<D, HL_FP8>(high, pp) : tile_kv<D, HL_BF16>(high, pp));
 }
 }  // namespace
+
+namespace {
+template <int KVT>
+ChunkBothFn both_kv(bool high, int rb) {
+  return high ? (rb == 1 ? chunk_both_kernel<64, KVT, true, 1> : chunk_both_kernel<64, KVT, true, 2>)
+              : (rb == 1 ? chunk_both_kernel<64, KVT, false, 1> : chunk_both_kernel<64, KVT, false, 2>);
+}
+}  // namespace
+ChunkBothFn chunk_both_fn(int kv_dtype, bool high, int rb) {
+  return kv_dtype == HL_F16 ? both_kv<HL_F16>(high, rb) : (kv_dtype == HL_FP8 ? both_kv<HL_FP8>(high, rb) : both_kv<HL_BF16>(high, rb));
+}
 
 ChunkFn chunk_tile_fn(int head_dim, int kv_dtype, bool high, bool pp) {
   return head_dim == 64 ? tile_d<64>(kv_dtype, high, pp) : tile_d<128>(kv_dtype, high, pp);

@@ -9,7 +9,7 @@ import pytest
 from hippo_leap_amd import build as hb
 from test_kernel_resources import _resources
 
-CHECKED = {"chunk.hip": "chunk_few_kernel", "chunk_tile.hip": "chunk_tile_kernel",
+CHECKED = {"chunk.hip": "chunk_few_kernel", "chunk_tile.hip": "_kernel",
            "rope_chunk.hip": "rope_chunk_kernel", "pages.hip": "pages_copy_kernel"}
 
 
