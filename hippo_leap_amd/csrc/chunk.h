@@ -363,9 +363,10 @@ __device__ __forceinline__ float merge_weight(float m, float M) { return m == M 
 // per workgroup of 8 (pp); high: fp32 precision.
 typedef void (*ChunkFn)(ChunkParams);
 ChunkFn chunk_tile_fn(int head_dim, int kv_dtype, bool high, bool pp);
-// Both kernels in one launch (head dim 64): workgroups of the flash kernel up
+// Both kernels in one launch (head dim 64, or 128 with 16-bit operands and
+// caches and without high; not pp): workgroups of the flash kernel up
 // to n_tile, then those of the few-rows kernel (its own parameters).
 typedef void (*ChunkBothFn)(ChunkParams p, ChunkParams few, int n_tile);
-ChunkBothFn chunk_both_fn(int kv_dtype, bool high, int rb);
+ChunkBothFn chunk_both_fn(int head_dim, int kv_dtype, bool high, int rb);
 
 }  // namespace hl

@@ -56,13 +56,16 @@ long long most_tiles(const hl_attn_chunk_args* a, int tokens) {
   const long long seen = ((long long)a->window + tokens + 30) / 32 + 1 + ((long long)a->n_sink + 31) / 32;
   return std::min(all, seen);
 }
-// Both kernels in one launch: at head dim 64, where their LDS leaves room for
-// two workgroups per CU.  The few-rows kernel's memory waits then run beside
-// the flash kernel's arithmetic: 26 sequences, chunks of up to 351 tokens and
-// single tokens over 3K, 84.4 -> 65.1 us with the same splits, 55.3 with those of this launch.  At 128 the
-// few-rows kernel's 128 KB would leave the flash kernel one workgroup per CU.
-bool chunk_both(int head_dim, const ChunkAttnPlan* plan) {
-  return plan->tile.items > 0 && plan->few.items > 0 && head_dim == 64;
+// Both kernels in one launch, where two workgroups per CU of either have room:
+// the few-rows kernel's memory waits then run beside the flash kernel's
+// arithmetic.  Not the 8-wave form; and at head dim 128 neither fp32's
+// precision nor fp8, whose registers do not allow two.  26 sequences, chunks of
+// up to 351 tokens and single tokens over 3K, head dim 64: 84.4 -> 65.1 us with
+// the same splits, 55.6 with those of this
+// launch; head dim 128, bf16: 129 -> 87.
+bool chunk_both(const hl_attn_chunk_args* a, const ChunkAttnPlan* plan) {
+  return plan->tile.items > 0 && plan->few.items > 0 && !plan->pp &&
+         (a->seqs.head_dim == 64 || (!plan->high && a->seqs.kv_dtype != HL_FP8));
 }
 }  // namespace
 
@@ -108,7 +111,7 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
     // tiles.  8 sequences at 2K, head dim 64 (us by splits): 1 19.7, 2 13.9,
     // 4 12.1, 8 12.9, 16 18.9; 16 windows of 4K, head dim 128: 2 33.9, 4 28.4,
     // 8 33.2.
-    const int resident = cu_count() * (D == 64 || s.kv_dtype == HL_FP8 ? 2 : 1);
+    const int resident = cu_count() * (D == 64 || s.kv_dtype == HL_FP8 || chunk_both(a, plan) ? 2 : 1);
     const bool fits = units <= kChunkSlots / 2;
     long long S = 1, best_cost = 0;
     for (long long n = 1; n <= (fits ? std::min<long long>((tiles + 3) / 4, 64) : 1); ++n) {
@@ -143,23 +146,22 @@ void chunk_attn_plan(const hl_attn_chunk_args* a, ChunkAttnPlan* plan) {
     const int cus = cu_count() * (plan->pp || (plan->high && D == 128) ? 1 : 2);
     const long long likely =
         s.n_head_kv * std::min<long long>(t.items, std::max(long_seqs, (int)(rows / t.rows) + (long_seqs + 1) / 2));
-    // In one launch with the few-rows kernel, whose workgroups come last: all
-    // work (a 64-key tile of theirs is worth one and a half), or the flash
-    // kernel's up to its last blocks, which are half through on average, and
-    // their other half (us by splits: 26 sequences of 3K, 4 of
-    // them chunks of 243 to 351: 1 57.8, 2 60.0, 4 66.7; 10 of 16K, chunks of 512 and
-    // 476: 1 228, 2 168, 4 160, 8 173; 64 of 2K, chunks of 100, 64 and 28: 1 47.5, 2
-    // 33.4, 4 33.2, 8 38.9).
-    const long long beside = chunk_both(D, plan) ? (long long)std::max(0, s.batch - long_seqs) * s.n_head_kv * tiles * 3 / 2 : 0;
+    // In one launch with the few-rows kernel, whose workgroups come last, their
+    // work (a 64-key tile of theirs is worth one and a half) fills up to half of
+    // what the last blocks leave of the GPU; the longest block is a bound of its
+    // own (us by splits: 26 sequences of 3K, 4 of them chunks of 243 to 351: 1
+    // 57.8, 2 60.0, 4 66.7; 10 of 16K, chunks of 512 and 476: 1 228, 2 168, 4 160,
+    // 8 173; 64 of 2K, chunks of 100, 64 and 28: 1 47.5, 2 33.4, 4 33.2, 8 38.9).
+    const long long beside = chunk_both(a, plan) ? (long long)std::max(0, s.batch - long_seqs) * s.n_head_kv * tiles * 3 / 2 : 0;
     long long best = 1, best_cost = 0;
     const bool fits = units * waves <= kChunkSlots / 2;
     const long long most = fits ? std::min<long long>({tiles, 32, std::max<long long>(1, 1536 / units)}) : 1;
     for (long long S = 1; S <= most; ++S) {
       const long long piece = (tiles + S - 1) / S + 4 + (S > 1 ? 8 : 0);
-      const long long work = likely * S * piece, half = piece * cus / 2;
-      const long long cost = chunk_both(D, plan) ? std::max(work + beside, std::max(work, half) + half)
+      const long long work = likely * S * piece, last = piece * cus;
+      const long long cost = chunk_both(a, plan) ? std::max({work + beside, last, work + last - std::min(beside, last / 2)})
                              : long_seqs == 1 ? (likely * S + cus - 1) / cus * piece * cus
-                                              : work + piece * cus;
+                                              : work + last;
       if (S == 1 || cost < best_cost) best = S, best_cost = cost;
     }
     if (a->num_splits > 0 && fits) best = std::min<long long>({a->num_splits, tiles, 256});
@@ -216,8 +218,8 @@ hipError_t chunk_attn_launch(const hl_attn_chunk_args* a, const ChunkAttnPlan* p
     n_wg[k] = (unsigned)(t.items * t.splits) * s.n_head_kv;
   }
   // The flash kernel's workgroups first: they are the longer ones.
-  if (chunk_both(D, plan)) {
-    hipLaunchKernelGGL(chunk_both_fn(s.kv_dtype, plan->high, plan->rb), dim3(n_wg[0] + n_wg[1]), dim3(256), 0, stream, own[0],
+  if (chunk_both(a, plan)) {
+    hipLaunchKernelGGL(chunk_both_fn(D, s.kv_dtype, plan->high, plan->rb), dim3(n_wg[0] + n_wg[1]), dim3(256), 0, stream, own[0],
                        own[1], (int)n_wg[0]);
     return hipGetLastError();
   }

@@ -109,18 +109,23 @@ __device__ __forceinline__ void chunk_finish(const ChunkParams& p, const ChunkSe
 // of its own in flight behind the one it computes, without barriers.  16
 // single tokens, head dim 128, fp32 on bf16: all of 32K 186 us (5.7 TB/s), a
 // window of 4096 32 us (4.2 TB/s); one token over 1024 keys 8.9 us.
-template <int D, int KVT, bool HIGH, int RB>
+// STAGES: tiles of a wave in LDS.  With one the next tile is asked for when
+// the tile is done with, and two workgroups per CU cover each other's waits: as
+// good or up to 9% slower than two stages and one workgroup at head dim 128 (8
+// sequences' 5 tokens over 2K, 8 kv heads 21.3 / 23.1 us, 4 kv heads 27.6 / 27.6), but
+// room for the flash kernel's workgroups beside it.  fp8 converts from
+// registers, which are its second stage.
+template <int D, int KVT, bool HIGH, int RB, int STAGES = KVT == HL_FP8 ? 1 : 2>
 struct ChunkFew {
   static constexpr int ROWS = 16 * RB, TILE = D * 32;  // TILE: elements of a K or V tile
-  static constexpr int STAGES = KVT == HL_FP8 ? 1 : 2;
   static constexpr int WAVE_ELEMS = STAGES * 2 * TILE;
   static constexpr int MERGE_BYTES = 4 * ROWS * (D + 4 + 2) * 4;
   static constexpr int LDS_BYTES = 4 * WAVE_ELEMS * 2 > MERGE_BYTES ? 4 * WAVE_ELEMS * 2 : MERGE_BYTES;
 };
-template <int D, int KVT, bool HIGH, int RB>
+template <int D, int KVT, bool HIGH, int RB, int STAGES = KVT == HL_FP8 ? 1 : 2>
 __device__ __forceinline__ void chunk_few(const ChunkParams& p, unsigned char* lds, int b, int kvh, int split) {
   typedef OpT<KVT> Op;
-  typedef ChunkFew<D, KVT, HIGH, RB> F;
+  typedef ChunkFew<D, KVT, HIGH, RB, STAGES> F;
   constexpr int MT = Op::dt;
   constexpr int NQ = HIGH ? (MT == HL_BF16 ? 3 : 2) : 1, NP = NQ;
   constexpr int KS = D / 32, NB = D / 16, ROWS = F::ROWS, TILE = F::TILE, WAVE_ELEMS = F::WAVE_ELEMS;
@@ -342,6 +347,14 @@ __device__ __forceinline__ void chunk_few(const ChunkParams& p, unsigned char* l
         compute(n, 0);
       }
       wave_lds_sync();
+    } else if constexpr (STAGES == 1) {
+      wait_vm<0>();
+      compute(n, 0);
+      if (n + 1 < n_tiles) {
+        if (((n + 1) & 63) == 0) load_pages(n + 1);
+        wait_lgkm();  // the stage's reads are done
+        request(n + 1, 0);
+      }
     } else {
       if (n + 1 < n_tiles) {
         const int keep = pages;

@@ -673,7 +673,8 @@ __global__ __launch_bounds__(PP ? 512 : 256, HIGH && D == 128 ? 1 : 2) void chun
 // Both kernels' workgroups in one launch, the flash kernel's first.
 template <int D, int KVT, bool HIGH, int RB>
 __global__ __launch_bounds__(256, 2) void chunk_both_kernel(ChunkParams p, ChunkParams few, int n_tile) {
-  constexpr int A = kTileLds<D, false> * 2, B = ChunkFew<D, KVT, HIGH, RB>::LDS_BYTES;
+  constexpr int STAGES = KVT == HL_FP8 || D == 128 ? 1 : 2;
+  constexpr int A = kTileLds<D, false> * 2, B = ChunkFew<D, KVT, HIGH, RB, STAGES>::LDS_BYTES;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[A > B ? A : B];
   int id = blockIdx.x;
   if (id < n_tile) {
@@ -683,7 +684,7 @@ __global__ __launch_bounds__(256, 2) void chunk_both_kernel(ChunkParams p, Chunk
   id -= n_tile;
   const int b = id % few.items;
   id /= few.items;
-  chunk_few<D, KVT, HIGH, RB>(few, lds, b, id % few.s.n_head_kv, id / few.s.n_head_kv);
+  chunk_few<D, KVT, HIGH, RB, STAGES>(few, lds, b, id % few.s.n_head_kv, id / few.s.n_head_kv);
 }
 
 namespace {
@@ -702,13 +703,17 @@ ChunkFn tile_d(int kv, bool high, bool pp) {
 
 namespace {
 template <int KVT>
-ChunkBothFn both_kv(bool high, int rb) {
+ChunkBothFn both_kv(int head_dim, bool high, int rb) {
+  if constexpr (KVT != HL_FP8)
+    if (head_dim == 128)
+      return rb == 1 ? chunk_both_kernel<128, KVT, false, 1> : chunk_both_kernel<128, KVT, false, 2>;
   return high ? (rb == 1 ? chunk_both_kernel<64, KVT, true, 1> : chunk_both_kernel<64, KVT, true, 2>)
               : (rb == 1 ? chunk_both_kernel<64, KVT, false, 1> : chunk_both_kernel<64, KVT, false, 2>);
 }
 }  // namespace
-ChunkBothFn chunk_both_fn(int kv_dtype, bool high, int rb) {
-  return kv_dtype == HL_F16 ? both_kv<HL_F16>(high, rb) : (kv_dtype == HL_FP8 ? both_kv<HL_FP8>(high, rb) : both_kv<HL_BF16>(high, rb));
+ChunkBothFn chunk_both_fn(int head_dim, int kv_dtype, bool high, int rb) {
+  return kv_dtype == HL_F16 ? both_kv<HL_F16>(head_dim, high, rb)
+                            : (kv_dtype == HL_FP8 ? both_kv<HL_FP8>(head_dim, high, rb) : both_kv<HL_BF16>(head_dim, high, rb));
 }
 
 ChunkFn chunk_tile_fn(int head_dim, int kv_dtype, bool high, bool pp) {

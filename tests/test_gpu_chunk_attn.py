@@ -216,6 +216,24 @@ def test_contexts_beyond_the_page_table_in_lds(hl, new, io, kv):
         check_attn(c, hidden_pages=(7, 4000))
 
 
+@pytest.mark.parametrize("splits", [0, 1, 3])
+@pytest.mark.parametrize("d,io,kv", [(64, "bf16", "bf16"), (64, "f32", "f16"), (64, "f16", "fp8"), (128, "bf16", "bf16"),
+                                     (128, "f16", "f16"), (128, "f32", "bf16"), (128, "bf16", "fp8")])
+def test_single_tokens_beside_chunks(hl, d, io, kv, splits):
+    """One token over more than 64 tiles per wave beside chunks, in one launch or two;
+    pages missing in both; groups of 16 and of 17 to 32 rows."""
+    from hippo_leap_amd import attention as A
+    for hq in (8, 32):
+        print(f"beside {d} {io} {kv} {splits} {hq}", flush=True)
+        c = Case([1, 100, 1, 0, 41, 1], [9001, 700, 8300, 5, 41, 1], hq, 1, d, io, kv, seed=hq)
+        c.table[:, 2] = -1
+        c.table[0, 270] = c.n_pages
+        for _ in range(2):
+            c.out.fill_(77)
+            c.run_attn(A, num_splits=splits)
+            check_attn(c, hidden_pages=(2, 270))
+
+
 def test_missing_pages_in_the_eight_wave_form(hl):
     from hippo_leap_amd import attention as A
     for kv in ("bf16", "fp8"):
