@@ -152,9 +152,11 @@ struct OpT<HL_BF16> {
 // register.  Written out, because behind the builtin the compiler waits for
 // every copy in flight before any LDS read, whichever stage it reads (here a
 // stage's copies are waited for by count, wait_vm): 2048 tokens over 16K, head
-// dim 128, 566 -> 521 us; 16 sequences' single tokens 38.5 -> 35.4.
+// dim 128, 566 -> 521 us; 16 sequences' single tokens 38.5 -> 35.4.  The wait
+// states are those that an address which a vector instruction wrote to its
+// scalar registers needs (five); the compiler does not see the load in here.
 __device__ __forceinline__ void copy16_to_lds(const void* base, unsigned lane_bytes, unsigned lds_at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(lds_at), "v"(lane_bytes), "s"((uint64_t)(uintptr_t)base)
                : "memory", "m0");
